@@ -134,6 +134,11 @@ SIGNATURES = {
     "hf2q_cuda_ssd_prep": (i32, [vp, vp, vp, u32, vp, vp, vp]),
     "hf2q_cuda_ssd_scan": (i32, [vp, vp, vp, u32, vp, vp, vp, vp]),
     "hf2q_cuda_state_tail": (i32, [vp, vp, vp, u32, vp, vp, u32, vp]),
+    "hf2q_cuda_pages_append": (i32, [vp, vp, vp, vp, vp, vp, u32, u32, u32, vp, u32, u32]),
+    "hf2q_cuda_pages_attend_scratch_bytes": (i32, [vp, vp, vp, u32, u32, u32, C.POINTER(u64)]),
+    "hf2q_cuda_pages_attend": (i32, [vp, vp, vp, vp, vp, u32, u32, u32, C.c_float, u32, u32, vp, u32, u32, vp, u64]),
+    "hf2q_cuda_pages_copy": (i32, [vp, vp, vp, u32, vp, vp, u32]),
+    "hf2q_cuda_pages_copy_rows": (i32, [vp, vp, vp, u32, vp, vp, u32]),
     "hf2q_cuda_launch_count": (u64, [vp]),
     "hf2q_cuda_sm_count": (i32, [vp]),
     "hf2q_cuda_version": (C.c_char_p, []),

@@ -260,6 +260,7 @@ HF2Q_API int32_t hf2q_cuda_check_status(hf2q_ctx* ctx, void* stream) {
     if (e != cudaSuccess) return cuda_fail(ctx, e, "status read-back");
     if (word & STATUS_WAIT_TIMEOUT) return fail(ctx, HF2Q_ERR_TIMEOUT, "a kernel gave up a bounded wait (status 0x%x)", word);
     if (word & STATUS_BAD_EXPERT_ID) return fail(ctx, HF2Q_ERR_INVALID_ARGUMENT, "ids[] held an expert index >= n_experts (status 0x%x)", word);
+    if (word & STATUS_BAD_PAGE) return fail(ctx, HF2Q_ERR_INVALID_ARGUMENT, "a page, row, length or start of a paged call was out of range (status 0x%x)", word);
     if (word & STATUS_X_CLIPPED) return fail(ctx, HF2Q_ERR_INVALID_ARGUMENT, "an activation exceeded 65504 in magnitude and was clipped (status 0x%x)", word);
     return HF2Q_OK;
 }

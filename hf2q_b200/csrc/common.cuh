@@ -22,6 +22,7 @@ enum : uint32_t {
     STATUS_WAIT_TIMEOUT = 1u,   // a bounded mbarrier wait gave up
     STATUS_BAD_EXPERT_ID = 2u,  // ids[] held a value >= n_experts
     STATUS_X_CLIPPED = 4u,      // an activation exceeded the f16 range (65504) and was clipped
+    STATUS_BAD_PAGE = 8u,       // a page, row, length or start of a paged call was out of range
 };
 
 struct BlockGeom { uint32_t elems, bytes; };

@@ -1,0 +1,92 @@
+// What the kernels of the paged cache share: the views that a launch gets by value, and how a sequence's rows and positions are found
+// on the device.  Every number that comes from device memory is checked before it becomes an address.
+#pragma once
+#include <cstdio>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace hf2q {
+namespace paged {
+
+// one layer's pool
+struct Pool {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    uint32_t pages, shift, kv_heads;         // page size 1 << shift
+    __host__ __device__ uint32_t size() const { return 1u << shift; }
+    // first row of head `head` in page `page`, in rows
+    __host__ __device__ size_t row(uint32_t page, uint32_t head, uint32_t in_page) const { return ((static_cast<size_t>(page) * kv_heads + head) << shift) + in_page; }
+};
+
+struct Batch {
+    const uint32_t *start, *length, *table;
+    uint32_t seqs, rows, table_ld, max_new, max_length;
+};
+
+// The new rows of a sequence and the positions it holds; what does not fit is cut to what is safe and `bad` says so.
+struct Span {
+    uint32_t row0, rows, length;
+    bool bad;
+};
+__host__ __device__ __forceinline__ Span span_of(const Batch& b, uint32_t shift, uint32_t s) {
+    Span o;
+    const uint32_t r0 = b.start[s], r1 = b.start[s + 1], len = b.length[s];
+    const uint64_t held = static_cast<uint64_t>(b.table_ld) << shift;
+    const uint32_t room = held < b.max_length ? static_cast<uint32_t>(held) : b.max_length;
+    o.row0 = r0 < b.rows ? r0 : b.rows;
+    const uint32_t end = r1 < b.rows ? r1 : b.rows, n = end > o.row0 ? end - o.row0 : 0u;
+    o.rows = n < b.max_new ? n : b.max_new;
+    o.length = len < room ? len : room;
+    o.bad = r1 < r0 || r1 > b.rows || r1 - r0 > b.max_new || len > room || (r1 > r0 && len < r1 - r0);
+    return o;
+}
+
+// page that holds position p of sequence s (p below the span's length); a number out of range counts as page 0
+__host__ __device__ __forceinline__ uint32_t page_of(const Pool& c, const Batch& b, uint32_t s, uint32_t p, bool& bad) {
+    const uint32_t page = b.table[static_cast<size_t>(s) * b.table_ld + (p >> c.shift)];
+    if (page < c.pages) return page;
+    bad = true;
+    return 0;
+}
+
+// the checks that all entries share; 0 or the text of what is wrong
+inline const char* pages_error(const hf2q_pages* c) {
+    if (!c || !c->k || !c->v) return "null cache pointer";
+    if (c->dtype != HF2Q_DT_I8 && c->dtype != HF2Q_DT_BF16) return "the cache is of signed bytes (I8) or BF16";
+    if (c->dtype == HF2Q_DT_I8 && (!c->k_scale || !c->v_scale)) return "a cache of bytes needs its scales";
+    if (c->page < 16 || c->page > 256 || (c->page & (c->page - 1))) return "a page holds 16, 32, 64, 128 or 256 positions";
+    if (c->dim != 64 && c->dim != 128) return "heads are of 64 or 128 elements";
+    if (c->pages == 0 || c->kv_heads == 0 || c->kv_heads > 65535) return "a pool has 1 page or more and 1 to 65535 heads";
+    if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v) | reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) % 16)
+        return "the cache's arrays start on 16-byte boundaries";
+    return nullptr;
+}
+inline const char* batch_error(const hf2q_page_batch* b) {
+    if (!b || !b->start || !b->length || !b->table) return "null batch pointer";
+    if (b->seqs == 0 || b->seqs > 65535 || b->table_ld == 0) return "a batch has 1 to 65535 sequences and a table";
+    if (b->max_new > b->rows || b->max_length < b->max_new || b->max_length > 1u << 30) return "max_new is at most rows and max_length, max_length at most 2^30";
+    if (b->rows > 1u << 28) return "a batch has at most 2^28 rows";
+    return nullptr;
+}
+inline int32_t refuse(hf2q_ctx* ctx, const char* who, const char* what) {
+    char text[256];
+    snprintf(text, sizeof text, "%s: %s", who, what);
+    return ctx_fail(ctx, HF2Q_ERR_INVALID_ARGUMENT, text);
+}
+inline Pool pool_of(const hf2q_pages* c) {
+    return Pool{c->k, c->v, c->k_scale, c->v_scale, c->pages, static_cast<uint32_t>(__builtin_ctz(c->page)), c->kv_heads};
+}
+inline Batch batch_of(const hf2q_page_batch* b) { return Batch{b->start, b->length, b->table, b->seqs, b->rows, b->table_ld, b->max_new, b->max_length}; }
+
+struct OnDevice {                            // the context's device for the length of a call
+    int prev = -1;
+    explicit OnDevice(int dev) {
+        if (cudaGetDevice(&prev) != cudaSuccess || prev == dev) prev = -1;
+        else cudaSetDevice(dev);
+    }
+    ~OnDevice() { if (prev >= 0) cudaSetDevice(prev); }
+};
+
+}  // namespace paged
+}  // namespace hf2q

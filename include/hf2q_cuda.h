@@ -77,8 +77,8 @@ enum {
     HF2Q_TYPE_MLX_AFFINE4_GS32 = 1000
 };
 
-/* Element types of activations and of dequantised output. */
-enum { HF2Q_DT_F32 = 0, HF2Q_DT_F16 = 1, HF2Q_DT_BF16 = 2 };
+/* Element types of activations and of dequantised output; I8: codes of a paged cache. */
+enum { HF2Q_DT_F32 = 0, HF2Q_DT_F16 = 1, HF2Q_DT_BF16 = 2, HF2Q_DT_I8 = 3 };
 
 /* ---- context ------------------------------------------------------------------------------ */
 
@@ -923,6 +923,62 @@ HF2Q_API int32_t hf2q_cuda_ssd_scan(hf2q_ctx* ctx, void* stream, const hf2q_ssd*
  * convolution inputs -> delta->conv_state (delta NULL: none). */
 HF2Q_API int32_t hf2q_cuda_state_tail(hf2q_ctx* ctx, void* stream, const uint32_t* pos, uint32_t m, const float* h_last,
                                       float* shift_state, uint32_t width, const hf2q_delta* delta);
+
+/* ---- a cache in pages: append, attention, moving ------------------------------------------------------ *
+ * Many sequences share one pool of pages; a sequence is a row of page numbers and a length.  One layer's pool: keys and values
+ * [pages][kv_heads][page][dim], bf16, or signed bytes with one f32 scale per (page, head, row) (value = code * scale, scale =
+ * amax / 127: the codes of hf2q_kv_cache).  page: 16, 32, 64, 128 or 256 positions; dim: 64 or 128; all arrays on 16-byte
+ * boundaries.  Offsets are 64-bit. */
+typedef struct hf2q_pages {
+    void *k, *v;
+    float *k_scale, *v_scale;    /* [pages][kv_heads][page], I8 only */
+    uint32_t pages, page, kv_heads, dim, dtype;
+} hf2q_pages;
+/* The rows of one call.  Sequence s owns rows start[s] .. start[s + 1] - 1 (possibly none) and holds length[s] positions, the new ones
+ * included: its rows are the last of them, in order.  Position p is row p % page of page table[s][p / page].  The arrays are read on
+ * the device, so that a captured call can be replayed on other values; the call itself is laid out for `rows` rows in all, at most
+ * max_new rows and max_length positions of a sequence.  Rows behind start[seqs] are left as they were.  What does not fit (a
+ * page number >= pages, a length above max_length or the table, more than max_new rows, a row before position 0, starts that run
+ * backwards or past `rows`) touches no memory outside the arrays and is reported by hf2q_cuda_check_status; the outputs of the
+ * sequences that it concerns mean nothing. */
+typedef struct hf2q_page_batch {
+    const uint32_t *start, *length, *table;
+    uint32_t seqs, rows, table_ld, max_new, max_length;
+} hf2q_page_batch;
+/* Rotary turn: the first rot_dim elements of a head (even, <= dim) in pairs, (2i, 2i + 1) or with halves != 0 (i, i + rot_dim / 2), by
+ * position * freq[i] radians (product, sine and cosine in 64 bits), the result times factor.  freq f32 [rot_dim / 2]: any
+ * scaling for long contexts is in the table.  pos: position of each row [rows] (NULL: its position in its sequence). */
+typedef struct hf2q_rotary {
+    const float* freq;
+    const uint32_t* pos;
+    uint32_t rot_dim, halves;
+    float factor;
+} hf2q_rotary;
+/* Rows of x (f32 or bf16, ldx elements apart): queries [heads][dim], keys [kv_heads][dim], values [kv_heads][dim].  Queries are
+ * turned and stored to q_out (f32 or bf16, rows ldq apart), keys are turned and stored with the values at their positions.
+ * rotary NULL: nothing is turned. */
+HF2Q_API int32_t hf2q_cuda_pages_append(hf2q_ctx* ctx, void* stream, const hf2q_pages* c, const hf2q_page_batch* b,
+                                        const hf2q_rotary* rotary, const void* x, uint32_t x_dtype, uint32_t ldx,
+                                        uint32_t heads, void* q_out, uint32_t q_dtype, uint32_t ldq);
+/* Attention of every row over its sequence's positions (appended before): out[row][heads][dim] = softmax(q . k * scale) . v; query
+ * head h reads KV head h / (heads / kv_heads).  Position j is visible to i when j <= i and, with window > 0, i - j < window or
+ * j < sinks.  A row that sees nothing is zero; what a row does not see has no part in it, infinities and NaN included.  q f32 or
+ * bf16, out f32, bf16 or f16 (beyond the f16 range clipped and noted in the status).  Codes are multiplied as exact f16 numbers
+ * with q in f16 (clipped and noted), bf16 keys with q in bf16; probabilities are rounded to the same type, sums are f32.
+ * scratch: 256-byte aligned, of hf2q_cuda_pages_attend_scratch_bytes; its contents need not be kept. */
+HF2Q_API int32_t hf2q_cuda_pages_attend_scratch_bytes(hf2q_ctx* ctx, const hf2q_pages* c, const hf2q_page_batch* b, uint32_t heads,
+                                                      uint32_t window, uint32_t sinks, uint64_t* out);
+HF2Q_API int32_t hf2q_cuda_pages_attend(hf2q_ctx* ctx, void* stream, const hf2q_pages* c, const hf2q_page_batch* b, const void* q,
+                                        uint32_t q_dtype, uint32_t ldq, uint32_t heads, float scale, uint32_t window,
+                                        uint32_t sinks, void* out, uint32_t out_dtype, uint32_t ldo, void* scratch,
+                                        uint64_t scratch_bytes);
+/* Moves inside the pools of `layers` layers, each directly behind the one before (c: the first): whole pages src[i] -> dst[i], or rows
+ * src[i] -> dst[i] (row r of page g is g * page + r), i < n.  No destination is a source or named twice.  A number out of
+ * range moves nothing and is reported by hf2q_cuda_check_status. */
+HF2Q_API int32_t hf2q_cuda_pages_copy(hf2q_ctx* ctx, void* stream, const hf2q_pages* c, uint32_t layers, const uint32_t* src,
+                                      const uint32_t* dst, uint32_t n);
+HF2Q_API int32_t hf2q_cuda_pages_copy_rows(hf2q_ctx* ctx, void* stream, const hf2q_pages* c, uint32_t layers, const uint32_t* src,
+                                           const uint32_t* dst, uint32_t n);
 
 /* ---- introspection ------------------------------------------------------------------------ */
 
