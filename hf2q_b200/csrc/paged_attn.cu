@@ -3,120 +3,84 @@
 //   out[i] = sum_j p[i, j] v[j] / sum_j p[i, j],   p[i, j] = exp(scale q[i] . k[j] - max_j(..)) over the positions j that row i sees:
 //   j <= i and, with a window, i - j < window or j < sinks.
 //
-// attend_kernel: a warp per row and query head, 32 positions at a time with a running maximum and sum, all in f32.
+// Two kernels: paged_step.cu for few rows of a sequence (warp-level products, bound by memory), paged_tiles.cu for many (tcgen05).  Here are
+// the choice between them, how positions are split, and the sum of the parts.
 #include <math_constants.h>
 
-#include <type_traits>
+#include <algorithm>
 
 #include "paged_common.cuh"
-#include "seq_common.cuh"
 
 namespace hf2q {
 using namespace paged;
 namespace {
 
-struct Look {                                // what a row sees, and the scale of its scores in units of log2
-    uint32_t window, sinks;
-    float scale;
-    __device__ bool sees(uint32_t i, uint32_t j) const { return j <= i && (window == 0 || i - j < window || j < sinks); }
-};
-
-template <typename OUT> __device__ __forceinline__ OUT out_value(float v, bool& clipped) {
-    if constexpr (std::is_same_v<OUT, float>) return v;
-    else if constexpr (std::is_same_v<OUT, __half>) return panel_f16(v, clipped);
-    else return __float2bfloat16_rn(v);
-}
-
-constexpr uint32_t ROW_WARPS = 4;
-template <int DIM, bool CODES, typename Q, typename OUT>
-__global__ void __launch_bounds__(ROW_WARPS * 32) attend_kernel(Pool c, Batch b, Look look, uint32_t heads, const Q* q, uint32_t ldq, OUT* out, uint32_t ldo, uint32_t* status) {
-    __shared__ float qs[ROW_WARPS][DIM];
+// out[row][head] = sum of the parts, each weighted by exp2(its maximum - the largest), over the same sum of their weights.  A warp per row
+// and head; the order is that of the parts.
+constexpr uint32_t JOIN_WARPS = 4;
+template <int DIM, typename OUT>
+__global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(Batch b, uint32_t heads, uint32_t chunks, const float* part, const float* part_ml, OUT* out, uint32_t ldo, uint32_t* status) {
     constexpr int V = DIM / 32;
-    const uint32_t s = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Span span = span_of(b, c.shift, s);
-    if (span.bad && threadIdx.x == 0 && blockIdx.x == 0) atomicOr(status, STATUS_BAD_PAGE);
-    const uint64_t unit = static_cast<uint64_t>(blockIdx.x) * ROW_WARPS + warp;
-    if (unit >= static_cast<uint64_t>(span.rows) * heads) return;
-    const uint32_t r = static_cast<uint32_t>(unit / heads), h = static_cast<uint32_t>(unit % heads), kvh = h / (heads / c.kv_heads);
-    const size_t row = span.row0 + r;
-    for (uint32_t d = lane; d < DIM; d += 32) qs[warp][d] = seq::to_f32(q[row * ldq + static_cast<size_t>(h) * DIM + d]) * look.scale;
-    __syncwarp();
-    const bool any = span.length + r >= span.rows;
-    const uint32_t i = any ? span.length - span.rows + r : 0;
-    float mx = -CUDART_INF_F, l = 0.f, acc[V] = {};
-    bool bad = false;
-    for (uint32_t j0 = 0; any && j0 <= i; j0 += 32) {
-        const uint32_t j = j0 + lane;
-        const bool seen = look.sees(i, j);
-        if (!__any_sync(0xffffffffu, seen)) continue;
-        float x = -CUDART_INF_F, vsc = 0.f;
-        size_t at = 0;
-        if (seen) {
-            at = c.row(page_of(c, b, s, j, bad), kvh, j & (c.size() - 1));
-            x = 0.f;
-            if constexpr (CODES) {
-                const int8_t* k = static_cast<const int8_t*>(c.k) + at * DIM;
-                for (int d = 0; d < DIM; ++d) x = fmaf(qs[warp][d], static_cast<float>(k[d]), x);
-                x *= c.k_scale[at];
-                vsc = c.v_scale[at];
-            } else {
-                const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(c.k) + at * DIM;
-                for (int d = 0; d < DIM; ++d) x = fmaf(qs[warp][d], __bfloat162float(k[d]), x);
-                vsc = 1.f;
-            }
-        }
-        float top = x;
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float to = fmaxf(mx, top), base = to == -CUDART_INF_F ? 0.f : to, corr = exp2f(mx - base), p = seen ? exp2f(x - base) : 0.f;
-        mx = to;
-        l = l * corr + p;
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t lane = threadIdx.x & 31;
+    const uint64_t unit = static_cast<uint64_t>(blockIdx.x) * JOIN_WARPS + (threadIdx.x >> 5);
+    const uint32_t end = min(b.start[b.seqs], b.rows), begin = b.start[0];
+    if (unit >= static_cast<uint64_t>(end) * heads || unit / heads < begin) return;
+    const float2* ml = reinterpret_cast<const float2*>(part_ml) + unit * chunks;
+    float m_all = -CUDART_INF_F;
+    for (uint32_t i = lane; i < chunks; i += 32) m_all = fmaxf(m_all, ml[i].x);
+    for (int o = 16; o > 0; o >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, o));
+    float acc[V] = {}, sum = 0.f;
+#pragma unroll 4
+    for (uint32_t i = 0; i < chunks; ++i) {
+        const float2 x = ml[i];
+        const float f = part_factor(x.x, x.y, m_all);
+        if (f == 0.f) continue;
+        sum += x.y * f;
+        const float* p = part + (unit * chunks + i) * DIM + V * lane;
 #pragma unroll
-        for (int e = 0; e < V; ++e) acc[e] *= corr;
-        for (uint32_t o = 0; o < 32; ++o) {
-            const size_t there = __shfl_sync(0xffffffffu, at, o);
-            const float w = __shfl_sync(0xffffffffu, p * vsc, o);
-            if (!__shfl_sync(0xffffffffu, seen, o)) continue;
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const size_t d = there * DIM + V * lane + e;
-                acc[e] = fmaf(w, CODES ? static_cast<float>(static_cast<const int8_t*>(c.v)[d]) : __bfloat162float(static_cast<const __nv_bfloat16*>(c.v)[d]), acc[e]);
-            }
-        }
+        for (int e = 0; e < V; ++e) acc[e] += p[e] * f;
     }
-    l = seq::warp_sum(l);
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
     bool clipped = false;
-    for (int e = 0; e < V; ++e) out[row * ldo + static_cast<size_t>(h) * DIM + V * lane + e] = out_value<OUT>(l == 0.f ? 0.f : acc[e] * inv, clipped);
+    OUT* to = out + unit / heads * ldo + unit % heads * DIM + V * lane;
+#pragma unroll
+    for (int e = 0; e < V; ++e) to[e] = out_value<OUT>(acc[e] * inv, clipped);
     if (clipped) atomicOr(status, STATUS_X_CLIPPED);
-    if (bad) atomicOr(status, STATUS_BAD_PAGE);
+}
+template <int DIM>
+cudaError_t launch_join(const AttendCall& a) {
+    const dim3 grid(static_cast<uint32_t>((static_cast<uint64_t>(a.b.rows) * a.heads + JOIN_WARPS - 1) / JOIN_WARPS)), block(JOIN_WARPS * 32);
+    if (a.out_dtype == HF2Q_DT_F32) return launch_pdl(join_kernel<DIM, float>, grid, block, 0, a.st, a.b, a.heads, a.chunks, a.part, a.part_ml, static_cast<float*>(a.out), a.ldo, a.status);
+    if (a.out_dtype == HF2Q_DT_F16) return launch_pdl(join_kernel<DIM, __half>, grid, block, 0, a.st, a.b, a.heads, a.chunks, a.part, a.part_ml, static_cast<__half*>(a.out), a.ldo, a.status);
+    return launch_pdl(join_kernel<DIM, __nv_bfloat16>, grid, block, 0, a.st, a.b, a.heads, a.chunks, a.part, a.part_ml, static_cast<__nv_bfloat16*>(a.out), a.ldo, a.status);
 }
 
-struct Call {
-    Pool c;
-    Batch b;
-    Look look;
-    uint32_t heads;
-    const void* q;
-    uint32_t ldq;
-    void* out;
-    uint32_t ldo;
-    uint32_t* status;
-    cudaStream_t st;
+// How a call is laid out, from the bounds that the host knows.
+struct Plan {
+    bool step;
+    uint32_t chunk, chunks;
+    uint64_t scratch;
 };
-template <int DIM, bool CODES, typename Q, typename OUT>
-cudaError_t launch(const Call& a) {
-    const uint64_t units = static_cast<uint64_t>(a.b.max_new) * a.heads;
-    attend_kernel<DIM, CODES, Q, OUT><<<dim3(static_cast<uint32_t>((units + ROW_WARPS - 1) / ROW_WARPS), a.b.seqs), ROW_WARPS * 32, 0, a.st>>>(
-        a.c, a.b, a.look, a.heads, static_cast<const Q*>(a.q), a.ldq, static_cast<OUT*>(a.out), a.ldo, a.status);
-    return cudaGetLastError();
-}
-template <int DIM, bool CODES, typename Q>
-cudaError_t launch_out(const Call& a, uint32_t out_dtype) {
-    return out_dtype == HF2Q_DT_F32 ? launch<DIM, CODES, Q, float>(a) : out_dtype == HF2Q_DT_F16 ? launch<DIM, CODES, Q, __half>(a) : launch<DIM, CODES, Q, __nv_bfloat16>(a);
-}
-template <int DIM, bool CODES>
-cudaError_t launch_q(const Call& a, uint32_t q_dtype, uint32_t out_dtype) {
-    return q_dtype == HF2Q_DT_F32 ? launch_out<DIM, CODES, float>(a, out_dtype) : launch_out<DIM, CODES, __nv_bfloat16>(a, out_dtype);
+Plan plan_of(const hf2q_pages& c, const hf2q_page_batch& b, uint32_t heads, uint32_t window, uint32_t sinks, int sms) {
+    Plan p{};
+    const uint64_t group = heads / c.kv_heads, units = b.max_new * group;
+    p.step = true;
+    const uint64_t rows = units <= 8 ? 8 : 16;
+    // most positions that a tile goes through; and tiles, as if every sequence that can have rows had the most
+    uint64_t seen = (b.max_length + 127ull) / 128 * 128;
+    if (window) seen = std::min<uint64_t>(seen, (static_cast<uint64_t>(window) + b.max_new + sinks + 256 + 127) / 128 * 128);
+    const uint64_t tiles = static_cast<uint64_t>(c.kv_heads) * std::min(b.seqs, b.rows) * ((units + rows - 1) / rows);
+    // One part for each place that a CTA can have; several sequences are of several lengths, and smaller parts even them out.
+    const uint64_t places = 2ull * sms * (b.seqs > 1 ? 4 : 1);
+    uint64_t chunk = std::max<uint64_t>(256, (tiles * seen + places - 1) / places);
+    chunk = std::max(chunk, (seen + 255) / 256);
+    chunk = (chunk + 127) / 128 * 128;
+    p.chunks = static_cast<uint32_t>((seen + chunk - 1) / chunk);
+    p.chunk = static_cast<uint32_t>(chunk);
+    p.scratch = p.chunks > 1 ? (static_cast<uint64_t>(b.rows) * heads * p.chunks * (c.dim + 2) * 4 + 255) / 256 * 256 : 256;
+    return p;
 }
 
 const char* heads_error(const hf2q_pages* c, uint32_t heads) {
@@ -137,7 +101,7 @@ HF2Q_API int32_t hf2q_cuda_pages_attend_scratch_bytes(hf2q_ctx* ctx, const hf2q_
     if (const char* e = batch_error(b)) return refuse(ctx, who, e);
     if (const char* e = heads_error(c, heads)) return refuse(ctx, who, e);
     if (!out) return refuse(ctx, who, "null pointer");
-    *out = 256;
+    *out = plan_of(*c, *b, heads, window, sinks, ctx_sm_count(ctx)).scratch;
     return HF2Q_OK;
 }
 
@@ -155,15 +119,16 @@ HF2Q_API int32_t hf2q_cuda_pages_attend(hf2q_ctx* ctx, void* stream, const hf2q_
     if (ldq < width || ldo < width) return refuse(ctx, who, "rows overlap (ldq or ldo is too small)");
     if (reinterpret_cast<uintptr_t>(q) % (q_dtype == HF2Q_DT_F32 ? 4 : 2) || reinterpret_cast<uintptr_t>(out) % (out_dtype == HF2Q_DT_F32 ? 4 : 2)) return refuse(ctx, who, "rows start between two elements");
     if (b->rows == 0 || b->max_new == 0) return HF2Q_OK;
-    uint64_t need = 0;
-    if (const int32_t rc = hf2q_cuda_pages_attend_scratch_bytes(ctx, c, b, heads, window, sinks, &need)) return rc;
-    if (!scratch || scratch_bytes < need) return ctx_fail(ctx, HF2Q_ERR_WORKSPACE, "pages_attend: scratch missing or too small (ask hf2q_cuda_pages_attend_scratch_bytes)");
+    const Plan p = plan_of(*c, *b, heads, window, sinks, ctx_sm_count(ctx));
+    if (!scratch || scratch_bytes < p.scratch) return ctx_fail(ctx, HF2Q_ERR_WORKSPACE, "pages_attend: scratch missing or too small (ask hf2q_cuda_pages_attend_scratch_bytes)");
     if (reinterpret_cast<uintptr_t>(scratch) % 256) return refuse(ctx, who, "scratch is 256-byte aligned");
     const OnDevice on(ctx_device(ctx));
-    const Call a{pool_of(c), batch_of(b), Look{window, sinks, scale * 1.4426950408889634f}, heads, q, ldq, out, ldo, ctx_status_word(ctx), static_cast<cudaStream_t>(stream)};
-    const bool codes = c->dtype == HF2Q_DT_I8;
-    const auto go = c->dim == 128 ? (codes ? launch_q<128, true> : launch_q<128, false>) : (codes ? launch_q<64, true> : launch_q<64, false>);
-    return ctx_cuda_result(ctx, go(a, q_dtype, out_dtype), who, 1);
+    float* part = static_cast<float*>(scratch);
+    const AttendCall a{pool_of(c), batch_of(b), Look{window, sinks, scale * 1.4426950408889634f}, heads, q, q_dtype, ldq, out, out_dtype, ldo, p.chunk, p.chunks,
+                       part, part + static_cast<size_t>(b->rows) * heads * p.chunks * c->dim, ctx_status_word(ctx), static_cast<cudaStream_t>(stream)};
+    cudaError_t e = launch_attend_step(a, c->dim, c->dtype == HF2Q_DT_I8);
+    if (e == cudaSuccess && p.chunks > 1) e = c->dim == 128 ? launch_join<128>(a) : launch_join<64>(a);
+    return ctx_cuda_result(ctx, e, who, p.chunks > 1 ? 2 : 1);
 }
 
 }  // extern "C"

@@ -38,7 +38,7 @@ __host__ __device__ __forceinline__ Span span_of(const Batch& b, uint32_t shift,
     const uint32_t end = r1 < b.rows ? r1 : b.rows, n = end > o.row0 ? end - o.row0 : 0u;
     o.rows = n < b.max_new ? n : b.max_new;
     o.length = len < room ? len : room;
-    o.bad = r1 < r0 || r1 > b.rows || r1 - r0 > b.max_new || len > room || (r1 > r0 && len < r1 - r0);
+    o.bad = r1 < r0 || r1 > b.rows || r1 - r0 > b.max_new || len > room;
     return o;
 }
 
@@ -49,6 +49,62 @@ __host__ __device__ __forceinline__ uint32_t page_of(const Pool& c, const Batch&
     bad = true;
     return 0;
 }
+
+// What a row sees, and the scale of its scores in units of log2.
+struct Look {
+    uint32_t window, sinks;
+    float scale;
+    __host__ __device__ bool sees(uint32_t i, uint32_t j) const { return j <= i && (window == 0 || i - j < window || j < sinks); }
+};
+
+// The blocks of `unit` positions (unit = 1 << log) that rows at positions first .. last see, numbered without a gap: those of the first
+// positions, then those from the window's lower end of the first row to the last row.
+struct Blocks {
+    uint32_t sinks, from, count;             // blocks of the first positions; first block of the window; all
+    __host__ __device__ uint32_t at(uint32_t t) const { return t < sinks ? t : t - sinks + from; }
+};
+__host__ __device__ __forceinline__ Blocks blocks_of(const Look& k, uint32_t first, uint32_t last, uint32_t log) {
+    Blocks o;
+    o.from = (k.window && first >= k.window ? first - k.window + 1 : 0) >> log;
+    const uint64_t s = k.window ? (static_cast<uint64_t>(k.sinks) + (1u << log) - 1) >> log : 0;
+    o.sinks = s < o.from ? static_cast<uint32_t>(s) : o.from;
+    o.count = o.sinks + (last >> log) + 1 - o.from;
+    return o;
+}
+// every row at first .. last sees all of positions p .. p + n - 1; some row sees position p
+__host__ __device__ __forceinline__ bool all_see(const Look& k, uint32_t first, uint32_t last, uint32_t p, uint32_t n) {
+    return p + n - 1 <= first && (k.window == 0 || last - p < k.window || p + n <= k.sinks);
+}
+__host__ __device__ __forceinline__ bool some_see(const Look& k, uint32_t first, uint32_t last, uint32_t p) {
+    return p <= last && (k.window == 0 || p >= first || first - p < k.window || p < k.sinks);
+}
+
+// One attention call as the launchers take it.  With chunks > 1 a sequence's positions are split: part `chunk` of row and head leaves its
+// sum of weighted values (f32 [dim]) and (maximum, sum of weights) in scratch, and join_kernel adds the parts up in order.
+struct AttendCall {
+    Pool c;
+    Batch b;
+    Look look;
+    uint32_t heads;
+    const void* q;
+    uint32_t q_dtype, ldq;
+    void* out;
+    uint32_t out_dtype, ldo;
+    uint32_t chunk, chunks;                  // positions of a part, a multiple of 128
+    float *part, *part_ml;                   // [rows][heads][chunks][dim], [rows][heads][chunks][2]
+    uint32_t* status;
+    cudaStream_t st;
+};
+cudaError_t launch_attend_step(const AttendCall& a, uint32_t dim, bool codes);       // paged_step.cu
+cudaError_t launch_attend_tiles(const AttendCall& a, uint32_t dim, bool codes);      // paged_tiles.cu
+
+// what the sums of a part count for beside others: a part that saw nothing has none (its sum is 0), one of NaN scores alone has no maximum
+__device__ __forceinline__ float part_factor(float m, float l, float m_all) { return l == 0.f ? 0.f : m == -INFINITY ? 1.0f : exp2f(m - m_all); }
+
+template <typename OUT> __device__ __forceinline__ OUT out_value(float v, bool& clipped);
+template <> __device__ __forceinline__ float out_value<float>(float v, bool&) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 out_value<__nv_bfloat16>(float v, bool&) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half out_value<__half>(float v, bool& clipped) { return panel_f16(v, clipped); }      // (the panel of a product that follows)
 
 // the checks that all entries share; 0 or the text of what is wrong
 inline const char* pages_error(const hf2q_pages* c) {
