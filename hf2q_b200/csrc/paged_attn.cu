@@ -58,6 +58,7 @@ cudaError_t launch_join(const AttendCall& a) {
 }
 
 // How a call is laid out, from the bounds that the host knows.
+constexpr uint64_t STEP_UNITS = 32;          // rows of a sequence (tokens times heads of a group) that the step kernel takes
 struct Plan {
     bool step;
     uint32_t chunk, chunks;
@@ -66,15 +67,16 @@ struct Plan {
 Plan plan_of(const hf2q_pages& c, const hf2q_page_batch& b, uint32_t heads, uint32_t window, uint32_t sinks, int sms) {
     Plan p{};
     const uint64_t group = heads / c.kv_heads, units = b.max_new * group;
-    p.step = true;
-    const uint64_t rows = units <= 8 ? 8 : 16;
+    p.step = units <= STEP_UNITS;
+    const uint64_t rows = units <= 8 ? 8 : p.step ? 16 : 2 * (128 / group) * group;
     // most positions that a tile goes through; and tiles, as if every sequence that can have rows had the most
     uint64_t seen = (b.max_length + 127ull) / 128 * 128;
     if (window) seen = std::min<uint64_t>(seen, (static_cast<uint64_t>(window) + b.max_new + sinks + 256 + 127) / 128 * 128);
     const uint64_t tiles = static_cast<uint64_t>(c.kv_heads) * std::min(b.seqs, b.rows) * ((units + rows - 1) / rows);
     // One part for each place that a CTA can have; several sequences are of several lengths, and smaller parts even them out.
-    const uint64_t places = 2ull * sms * (b.seqs > 1 ? 4 : 1);
-    uint64_t chunk = std::max<uint64_t>(256, (tiles * seen + places - 1) / places);
+    const uint64_t places = (p.step ? 2ull : 1ull) * sms * (b.seqs > 1 && p.step ? 4 : 1);
+    uint64_t chunk = std::max<uint64_t>(p.step ? 256 : 512, (tiles * seen + places - 1) / places);
+    if (!p.step && tiles >= places) chunk = seen;
     chunk = std::max(chunk, (seen + 255) / 256);
     chunk = (chunk + 127) / 128 * 128;
     p.chunks = static_cast<uint32_t>((seen + chunk - 1) / chunk);
@@ -126,7 +128,7 @@ HF2Q_API int32_t hf2q_cuda_pages_attend(hf2q_ctx* ctx, void* stream, const hf2q_
     float* part = static_cast<float*>(scratch);
     const AttendCall a{pool_of(c), batch_of(b), Look{window, sinks, scale * 1.4426950408889634f}, heads, q, q_dtype, ldq, out, out_dtype, ldo, p.chunk, p.chunks,
                        part, part + static_cast<size_t>(b->rows) * heads * p.chunks * c->dim, ctx_status_word(ctx), static_cast<cudaStream_t>(stream)};
-    cudaError_t e = launch_attend_step(a, c->dim, c->dtype == HF2Q_DT_I8);
+    cudaError_t e = (p.step ? launch_attend_step : launch_attend_tiles)(a, c->dim, c->dtype == HF2Q_DT_I8);
     if (e == cudaSuccess && p.chunks > 1) e = c->dim == 128 ? launch_join<128>(a) : launch_join<64>(a);
     return ctx_cuda_result(ctx, e, who, p.chunks > 1 ? 2 : 1);
 }
