@@ -39,11 +39,19 @@ __device__ __forceinline__ uint32_t claim_columns(uint32_t* slot) {       // by 
     tmem_relinquish();
     return 0;
 }
+__device__ __forceinline__ bool elected() {                               // one lane of a whole warp
+    uint32_t yes;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+    return yes != 0;
+}
+// The bounded wait with its loop out of line: what every role goes through stays small (the instruction cache of a scheduler serves four roles).
+__device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity, uint32_t* status) { return mbar_wait_slow<0>(bar, parity, status); }
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, uint32_t* status) { return mbar_try_wait(bar, parity) || wait_on(bar, parity, status); }
 // all loader warps have come here for the n-th time (false: the wait ran out)
 __device__ __forceinline__ bool loaders_meet(uint64_t* bar, uint32_t n, uint32_t lane, uint32_t* status) {
     __syncwarp();
     if (lane == 0) mbar_arrive(bar);
-    return __all_sync(0xffffffffu, mbar_wait_bounded(bar, n & 1, status));
+    return __all_sync(0xffffffffu, wait(bar, n & 1, status));
 }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes) {       // zeros past `bytes`
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -140,7 +148,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
     __shared__ uint32_t s_odd[2];
     __shared__ uint64_t k_full[2], v_full[2], k_free[2], v_free[2], sc_full[SLOTS], s_full[2], p_full[2], o_done[2], meet;
     __shared__ uint32_t tmem_slot;
-    const uint32_t kvh = blockIdx.x % c.kv_heads, chunk = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t kvh = blockIdx.x % c.kv_heads, chunk = blockIdx.y, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     uint32_t seq = 0, tok0 = 0;
     if (!find_tile(b, c.shift, 2 * sh.tokens, (gridDim.x - 1 - blockIdx.x) / c.kv_heads, seq, tok0)) return;      // (the tiles with the most positions first)
     const Span span = span_of(b, c.shift, seq);
@@ -214,35 +222,38 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
         constexpr uint32_t ROW = DIM * (CODES ? 1 : 2);
         const uint32_t tid = threadIdx.x - SOFTMAX_WARPS * 32, ch = tid % CH, row0 = tid / CH, last16 = last & ~15u;
         bool bad = false, ok = true;
-        // lane g holds the page of positions 16 g .. 16 g + 15 of a block; positions past the last one repeat the last sixteen
-        auto pages_of = [&](uint32_t j) { return lane < BP / 16 ? page_of(c, b, seq, min((blocks.at(lo + j) << BP_LOG) + 16 * lane, last16), bad) : 0u; };
-        auto row_at = [&](uint32_t ids, uint32_t p0, uint32_t row) {
-            const uint32_t page = __shfl_sync(0xffffffffu, ids, row >> 4), p = min(p0 + (row & ~15u), last16) + (row & 15);
-            return c.row(page, kvh, p & (c.size() - 1));
+        // lane g holds where positions 16 g .. 16 g + 15 of a block lie, in sixteens of rows; positions past the last one repeat the last sixteen
+        auto places = [&](uint32_t j) {
+            const uint32_t p = min((blocks.at(lo + j) << BP_LOG) + 16 * (lane & 7), last16);
+            return static_cast<uint32_t>(c.row(page_of(c, b, seq, p, bad), kvh, p & (c.size() - 1)) >> 4);
         };
-        uint32_t ids = pages_of(0), next_ids = nb > 1 ? pages_of(1) : ids;
+        auto group = [&](uint32_t i) { return RP <= 16 ? RP * i >> 4 : (RP * i + row0) >> 4; };
+        auto place = [&](const void* array, uint32_t at16, uint32_t i, uint32_t row_bytes) {      // this thread's chunk of pass i
+            return static_cast<const uint8_t*>(array) + static_cast<uint64_t>(__shfl_sync(0xffffffffu, at16, group(i))) * (16 * row_bytes) + ((RP * i + row0) & 15) * row_bytes + 16 * ch;
+        };
+        uint32_t here = places(0), there = nb > 1 ? places(1) : here;
         if constexpr (CODES) {
             uint4 kq[NP], vq[NP];
             // every warp holds the scales of the whole block, four positions a lane, for the largest of V's; a quarter of the lanes stores
             float4 k4, v4;
             float unit = 0x1p-100f;
-            auto scales = [&](uint32_t id, uint32_t p0) {
-                const size_t r = row_at(id, p0, 4 * lane);
+            auto scales = [&](uint32_t at16) {
+                const uint64_t r = static_cast<uint64_t>(__shfl_sync(0xffffffffu, at16, lane >> 2)) * 16 + (4 * lane & 15);
                 k4 = __ldcg(reinterpret_cast<const float4*>(c.k_scale + r));
                 v4 = __ldcg(reinterpret_cast<const float4*>(c.v_scale + r));
             };
-            auto load = [&](const void* from, uint32_t id, uint32_t p0, uint4 (&x)[NP]) {
+            auto load = [&](const void* from, uint32_t at16, uint4 (&x)[NP]) {
 #pragma unroll
-                for (uint32_t i = 0; i < NP; ++i) x[i] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(from) + row_at(id, p0, RP * i + row0) * ROW) + ch);
+                for (uint32_t i = 0; i < NP; ++i) x[i] = __ldcg(reinterpret_cast<const uint4*>(place(from, at16, i, ROW)));
             };
             uint32_t p0 = blocks.at(lo) << BP_LOG;
-            load(c.k, ids, p0, kq);
-            scales(ids, p0);
-            load(c.v, ids, p0, vq);
+            load(c.k, here, kq);
+            scales(here);
+            load(c.v, here, vq);
             for (uint32_t j = 0; j < nb; ++j) {
                 const uint32_t st = j & 1, par = ((j >> 1) - 1) & 1, slot = j % SLOTS;
                 const uint32_t p1 = j + 1 < nb ? blocks.at(lo + j + 1) << BP_LOG : 0;
-                if (j >= 2) ok = mbar_wait_bounded(&k_free[st], par, status);
+                if (j >= 2) ok = wait(&k_free[st], par, status);
                 if (!__all_sync(0xffffffffu, ok)) break;
 #pragma unroll
                 for (uint32_t i = 0; i < NP; ++i) store_codes(ks + st * KV_BYTES, RP * i + row0, ch, kq[i]);
@@ -266,10 +277,10 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
                     mbar_arrive(&k_full[st]);
                 }
                 if (j + 1 < nb) {
-                    load(c.k, next_ids, p1, kq);
-                    scales(next_ids, p1);
+                    load(c.k, there, kq);
+                    scales(there);
                 }
-                if (j >= 2) ok = mbar_wait_bounded(&v_free[st], par, status);
+                if (j >= 2) ok = wait(&v_free[st], par, status);
                 if (!__all_sync(0xffffffffu, ok)) break;
 #pragma unroll
                 for (uint32_t i = 0; i < NP; ++i) store_codes(vs + st * KV_BYTES, RP * i + row0, ch, vq[i]);
@@ -277,33 +288,34 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&v_full[st]);
                 if (j + 1 < nb) {
-                    load(c.v, next_ids, p1, vq);
+                    load(c.v, there, vq);
                     p0 = p1;
-                    if (j + 2 < nb) next_ids = pages_of(j + 2);
+                    if (j + 2 < nb) there = places(j + 2);
                 }
             }
         } else {
-            auto copy = [&](const void* from, uint8_t* to, uint32_t id, uint32_t p0, bool zeros) {
+            const uint32_t to0 = chunk_at(row0, ch, PANEL);                  // (a pass is 8 rows or a multiple: the swizzle of a thread's chunk stays)
+            auto copy = [&](const void* from, uint8_t* to, uint32_t at16, uint32_t p0, bool zeros) {
+                const uint32_t dst = smem_u32(to) + to0;
 #pragma unroll
                 for (uint32_t i = 0; i < NP; ++i) {
-                    const uint32_t row = RP * i + row0;
-                    const bool take = !zeros || some_see(look, first, last, p0 + row);       // (values that nobody sees are zeros)
-                    copy16(smem_u32(to + chunk_at(row, ch, PANEL)), static_cast<const uint8_t*>(from) + row_at(id, p0, row) * ROW + 16 * ch, take ? 16 : 0);
+                    const bool take = !zeros || some_see(look, first, last, p0 + RP * i + row0);      // (values that nobody sees are zeros)
+                    copy16(dst + RP * i * 128, place(from, at16, i, ROW), take ? 16 : 0);
                 }
                 copies_close();
             };
             uint32_t p0 = blocks.at(lo) << BP_LOG;
-            copy(c.k, ks, ids, p0, false);
-            copy(c.v, vs, ids, p0, !all_see(look, first, last, p0, BP));
+            copy(c.k, ks, here, p0, false);
+            copy(c.v, vs, here, p0, !all_see(look, first, last, p0, BP));
             uint32_t met = 0;
             for (uint32_t j = 0; j < nb; ++j) {
                 const uint32_t st = j & 1, other = st ^ 1, par = ((j + 1) >> 1) - 1 & 1;
                 const bool more = j + 1 < nb;
                 const uint32_t p1 = more ? blocks.at(lo + j + 1) << BP_LOG : 0;
                 if (more) {
-                    if (j >= 1) ok = mbar_wait_bounded(&k_free[other], par, status);
+                    if (j >= 1) ok = wait(&k_free[other], par, status);
                     if (!__all_sync(0xffffffffu, ok)) break;
-                    copy(c.k, ks + other * KV_BYTES, next_ids, p1, false);
+                    copy(c.k, ks + other * KV_BYTES, there, p1, false);
                     copies_wait<2>();
                 } else copies_wait<1>();
                 proxy_fence();
@@ -331,57 +343,70 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&v_full[st]);
                 if (more) {
-                    if (j >= 1) ok = mbar_wait_bounded(&v_free[other], par, status);
+                    if (j >= 1) ok = wait(&v_free[other], par, status);
                     if (!__all_sync(0xffffffffu, ok)) break;
-                    copy(c.v, vs + other * KV_BYTES, next_ids, p1, !all_see(look, first, last, p1, BP));
+                    copy(c.v, vs + other * KV_BYTES, there, p1, !all_see(look, first, last, p1, BP));
                     p0 = p1;
-                    if (j + 2 < nb) next_ids = pages_of(j + 2);
+                    if (j + 2 < nb) there = places(j + 2);
                 }
             }
             copies_wait<0>();
         }
         if (bad) atomicOr(status, STATUS_BAD_PAGE);
-    } else if (warp == SOFTMAX_WARPS + LOAD_WARPS) {
-        if (lane == 0) {
-            // D f32; A and B f16 or bf16; M = 128; S: both K-major, N = 128; O: B MN-major, N = dim
+    } else if (warp >= SOFTMAX_WARPS + LOAD_WARPS) {
+        if (warp == SOFTMAX_WARPS + LOAD_WARPS) {
+            // D f32; A and B f16 or bf16; M = 128; S: both K-major, N = 128; O: B MN-major, N = dim.  The whole warp goes through the waits, so that
+            // addresses and descriptors stay in uniform registers; one lane issues.
             constexpr uint32_t ID = (1u << 4) | (CODES ? 0u : (1u << 7) | (1u << 10)) | ((ROWS >> 4) << 24), ID_S = ID | ((BP >> 3) << 17), ID_O = ID | (1u << 16) | ((DIM >> 3) << 17);
+            const uint32_t n = __shfl_sync(0xffffffffu, nb, 0), nt = __shfl_sync(0xffffffffu, tiles, 0), base = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint64_t q_desc = smem_desc_sw128(smem_u32(qs)), k_desc = smem_desc_sw128(smem_u32(ks)), v_desc = smem_desc_mn_sw128(smem_u32(vs), PANEL);
             bool ok = true;
-            auto scores = [&](uint32_t t, uint32_t j) {
-                const uint32_t st = j & 1;
-                if (t == 0) ok = mbar_wait_bounded(&k_full[st], (j >> 1) & 1, status);
-                if (ok && j) ok = mbar_wait_bounded(&o_done[t], (j - 1) & 1, status);        // P(j - 1) is read: S(j) takes its place
-                if (!ok) return;
-                tc_fence_after();
+            // (one place in the code for each product: S(j) of a tile behind its O += P(j - 1) V)
+            for (uint32_t j = 0; j <= n && ok; ++j) {
+                const uint32_t st = j & 1, was = st ^ 1;
+                for (uint32_t t = 0; t < nt && ok; ++t) {
+                    if (j) {
+                        if (t == 0) ok = wait(&v_full[was], ((j - 1) >> 1) & 1, status);
+                        if (ok) ok = wait(&p_full[t], (j - 1) & 1, status);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (elected()) {
+                            const uint64_t vd = v_desc + was * (KV_BYTES >> 4);
 #pragma unroll
-                for (uint32_t kk = 0; kk < DIM / 16; ++kk)
-                    umma_ss(tmem + t * BP, smem_desc_sw128(smem_u32(qs + t * Q_BYTES + (kk >> 2) * Q_PANEL)) + 2 * (kk & 3),
-                            smem_desc_sw128(smem_u32(ks + st * KV_BYTES + (kk >> 2) * PANEL)) + 2 * (kk & 3), ID_S, kk ? 1u : 0u);
-                tc_commit(&s_full[t]);
-                if (t + 1 == tiles) tc_commit(&k_free[st]);
-            };
-            for (uint32_t t = 0; t < tiles && ok; ++t) scores(t, 0);
-            for (uint32_t j = 0; j < nb && ok; ++j) {
-                const uint32_t st = j & 1;
-                for (uint32_t t = 0; t < tiles && ok; ++t) {
-                    if (t == 0) ok = mbar_wait_bounded(&v_full[st], (j >> 1) & 1, status);
-                    if (ok) ok = mbar_wait_bounded(&p_full[t], j & 1, status);
+                            for (uint32_t kk = 0; kk < BP / 16; ++kk) umma_ts(base + COL_O + t * DIM, base + t * BP + 8 * kk, vd + kk * (16 * 128 >> 4), ID_O, 1u);
+                            tc_commit(&o_done[t]);
+                            if (t + 1 == nt) tc_commit(&v_free[was]);
+                        }
+                        __syncwarp();
+                    }
+                    if (j == n) continue;
+                    if (t == 0) ok = wait(&k_full[st], (j >> 1) & 1, status);
+                    if (ok && j) ok = wait(&o_done[t], (j - 1) & 1, status);                  // P(j - 1) is read: S(j) takes its place
+                    ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after();
+                    if (elected()) {
+                        const uint64_t qd = q_desc + t * (Q_BYTES >> 4), kd = k_desc + st * (KV_BYTES >> 4);
 #pragma unroll
-                    for (uint32_t kk = 0; kk < BP / 16; ++kk)
-                        umma_ts(tmem + COL_O + t * DIM, tmem + t * BP + 8 * kk, smem_desc_mn_sw128(smem_u32(vs + st * KV_BYTES), PANEL) + kk * (16 * 128 >> 4), ID_O, 1u);
-                    tc_commit(&o_done[t]);
-                    if (t + 1 == tiles) tc_commit(&v_free[st]);
-                    if (j + 1 < nb) scores(t, j + 1);
+                        for (uint32_t kk = 0; kk < DIM / 16; ++kk)
+                            umma_ss(base + t * BP, qd + (kk >> 2) * (Q_PANEL >> 4) + 2 * (kk & 3), kd + (kk >> 2) * (PANEL >> 4) + 2 * (kk & 3), ID_S, kk ? 1u : 0u);
+                        tc_commit(&s_full[t]);
+                        if (t + 1 == nt) tc_commit(&k_free[st]);
+                    }
+                    __syncwarp();
                 }
             }
         }
-    } else if (warp / 4 < tiles) {
+    } else {
         const uint32_t tile = warp / 4, row = threadIdx.x & 127, at = tmem + (((warp & 3) * 32u) << 16), at_s = at + tile * BP, at_o = at + COL_O + tile * DIM;
         const uint32_t in_tile = row / sh.group, tile_tok = tok0 + tile * sh.tokens, tile_end = min(tile_tok + sh.tokens, end_tok), tok = tile_tok + in_tile;
         const bool live = in_tile < sh.tokens && tok < end_tok, held = live && tok >= lost;
         const uint32_t seen = before + max(min(tok, tile_end - 1), lost);          // (rows that are not there compute on zeros and are not stored)
         const uint32_t t_first = before + max(tile_tok, lost), t_last = before + max(tile_end - 1, lost);
+        // the row sees positions from `low` on, `reach` more, and those below `firsts`
+        const uint32_t low = !held ? 1u << 31 : look.window && seen >= look.window ? seen - look.window + 1 : 0, reach = held ? seen - low : 0;
+        const uint32_t firsts = held && look.window ? min(look.sinks, seen + 1) : 0;
         float mx = -CUDART_INF_F, unit = 0x1p-100f;
         f2 sum = 0;
         bool ok = true;
@@ -392,15 +417,16 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
 #pragma unroll
             for (uint32_t col = 0; col < DIM; col += 32) tmem_st32(at_o + col, zero);
         }
+        if (tile < tiles) {
         for (uint32_t j = 0; j < nb; ++j) {
             const uint32_t slot = j % SLOTS, st = j & 1, p0 = blocks.at(lo + j) << BP_LOG;
-            ok = mbar_wait_bounded(&s_full[tile], j & 1, status);
-            if constexpr (CODES) { if (ok) ok = mbar_wait_bounded(&sc_full[slot], (j / SLOTS) & 1, status); }
+            ok = wait(&s_full[tile], j & 1, status);
+            if constexpr (CODES) { if (ok) ok = wait(&sc_full[slot], (j / SLOTS) & 1, status); }
             const bool full = all_see(look, t_first, t_last, p0, BP) && tile_tok >= lost;
             bool odd = false;
             if constexpr (!CODES) {
                 if (!all_see(look, first, last, p0, BP) && first != last) {
-                    if (ok) ok = mbar_wait_bounded(&v_full[st], (j >> 1) & 1, status);
+                    if (ok) ok = wait(&v_full[st], (j >> 1) & 1, status);
                     odd = *static_cast<volatile uint32_t*>(&s_odd[st]) != 0;
                 }
             }
@@ -408,69 +434,66 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
             if (!ok) break;
             tc_fence_after();
             const ulonglong2 *k2 = reinterpret_cast<const ulonglong2*>(s_ks[slot]), *v2 = reinterpret_cast<const ulonglong2*>(s_vs[slot]);
-            const auto sees = [&](uint32_t p) { return held && look.sees(seen, p); };
-            // twice over the scores, 32 columns at a time: the maximum, then the exponentials
-            float top[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
-            auto largest = [&](auto masked) {
-#pragma unroll
-                for (uint32_t part32 = 0; part32 < BP / 32; ++part32) {
+            const auto sees = [&](uint32_t p) { return p - low <= reach || p < firsts; };
+            auto block = [&](auto masked) {
+                constexpr bool MASKED = decltype(masked)::value;
+                // twice over the scores, 32 columns at a time: the maximum, then the exponentials
+                float top[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll 1
+                for (uint32_t x = 0; x < BP / 32; ++x) {
                     uint32_t r[32];
-                    tmem_ld32(at_s + 32 * part32, r);
+                    tmem_ld32(at_s + 32 * x, r);
                     tmem_wait_ld();
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        float2 x = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-                        if constexpr (CODES) { const ulonglong2 k = k2[8 * part32 + i / 2]; x = f2_parts(f2_mul(f2_of(x.x, x.y), i & 1 ? k.y : k.x)); }
-                        if constexpr (decltype(masked)::value) {
-                            if (!sees(p0 + 32 * part32 + 2 * i)) x.x = -CUDART_INF_F;
-                            if (!sees(p0 + 32 * part32 + 2 * i + 1)) x.y = -CUDART_INF_F;
+                        float2 v = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+                        if constexpr (CODES) { const ulonglong2 k = k2[8 * x + i / 2]; v = f2_parts(f2_mul(f2_of(v.x, v.y), i & 1 ? k.y : k.x)); }
+                        if constexpr (MASKED) {
+                            if (!sees(p0 + 32 * x + 2 * i)) v.x = -CUDART_INF_F;
+                            if (!sees(p0 + 32 * x + 2 * i + 1)) v.y = -CUDART_INF_F;
                         }
-                        top[2 * (i & 1)] = fmaxf(top[2 * (i & 1)], x.x);
-                        top[2 * (i & 1) + 1] = fmaxf(top[2 * (i & 1) + 1], x.y);
+                        top[i & 3] = fmaxf(fmaxf(top[i & 3], v.x), v.y);
                     }
                 }
-            };
-            if (full) largest(std::false_type{}); else largest(std::true_type{});
-            float bm = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            if constexpr (!CODES) bm = bm == -CUDART_INF_F ? bm : bm * scale;
-            // the output is in units of `unit` times exp2 of the maximum
-            const float above = CODES ? s_unit[slot] : unit;
-            const bool grew = bm > mx + ROOM || (mx == -CUDART_INF_F && bm > mx);
-            if (__any_sync(0xffffffffu, grew || above != unit)) {
-                const float to = grew ? bm : mx;
-                float corr = grew ? ex2(mx - to) : 1.0f;
-                sum = f2_mul(sum, f2_both(corr));
-                mx = to;
-                corr *= unit / above;
-                unit = above;
-                if (j) {                                                  // (S(j) followed the output of block j - 1)
+                float bm = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                if constexpr (!CODES) bm = bm == -CUDART_INF_F ? bm : bm * scale;
+                // the output is in units of `unit` times exp2 of the maximum
+                const float above = CODES ? s_unit[slot] : unit;
+                const bool grew = bm > mx + ROOM || (mx == -CUDART_INF_F && bm > mx);
+                if (__any_sync(0xffffffffu, grew || above != unit)) {
+                    const float to = grew ? bm : mx;
+                    float corr = grew ? ex2(mx - to) : 1.0f;
+                    sum = f2_mul(sum, f2_both(corr));
+                    mx = to;
+                    corr *= unit / above;
+                    unit = above;
+                    if (j) {                                              // (S(j) followed the output of block j - 1)
 #pragma unroll 1
-                    for (uint32_t col = 0; col < DIM; col += 16) {
-                        uint32_t o[16];
-                        tmem_ld16(at_o + col, o);
-                        tmem_wait_ld();
+                        for (uint32_t col = 0; col < DIM; col += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(at_o + col, o);
+                            tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-                        tmem_st16(at_o + col, o);
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                            tmem_st16(at_o + col, o);
+                        }
                     }
                 }
-            }
-            const f2 nm = f2_both(mx == -CUDART_INF_F ? 0.f : -mx), sc2 = f2_both(scale);
-            auto weights = [&](auto masked) {
-#pragma unroll
-                for (uint32_t part32 = 0; part32 < BP / 32; ++part32) {
+                const f2 nm = f2_both(mx == -CUDART_INF_F ? 0.f : -mx), sc2 = f2_both(scale);
+#pragma unroll 1
+                for (uint32_t x = 0; x < BP / 32; ++x) {
                     uint32_t r[32], p[16];
-                    tmem_ld32(at_s + 32 * part32, r);
+                    tmem_ld32(at_s + 32 * x, r);
                     tmem_wait_ld();
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         f2 k = sc2;
-                        if constexpr (CODES) { const ulonglong2 kk = k2[8 * part32 + i / 2]; k = i & 1 ? kk.y : kk.x; }
+                        if constexpr (CODES) { const ulonglong2 kk = k2[8 * x + i / 2]; k = i & 1 ? kk.y : kk.x; }
                         float2 d = f2_parts(f2_fma(f2_of(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), k, nm));
                         bool s0 = true, s1 = true;
-                        if constexpr (decltype(masked)::value) {
-                            s0 = sees(p0 + 32 * part32 + 2 * i);
-                            s1 = sees(p0 + 32 * part32 + 2 * i + 1);
+                        if constexpr (MASKED) {
+                            s0 = sees(p0 + 32 * x + 2 * i);
+                            s1 = sees(p0 + 32 * x + 2 * i + 1);
                             if (!s0) d.x = -CUDART_INF_F;
                             if (!s1) d.y = -CUDART_INF_F;
                         }
@@ -478,16 +501,19 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
                         sum = f2_add(sum, e);
                         float2 w = f2_parts(e);
                         if constexpr (CODES) {
-                            const ulonglong2 v = v2[8 * part32 + i / 2];
+                            const ulonglong2 v = v2[8 * x + i / 2];
                             w = f2_parts(f2_mul(e, i & 1 ? v.y : v.x));
-                            if constexpr (decltype(masked)::value) { if (!s0) w.x = 0.f; if (!s1) w.y = 0.f; }
+                            if constexpr (MASKED) {                       // (also where the scale of V is infinite or NaN)
+                                if (!s0) w.x = 0.f;
+                                if (!s1) w.y = 0.f;
+                            }
                         }
                         p[i] = pack2<CODES>(w.x, w.y);
                     }
-                    tmem_st16(at_s + 16 * part32, p);                     // over scores that have been read
+                    tmem_st16(at_s + 16 * x, p);                          // over scores that have been read
                 }
             };
-            if (full) weights(std::false_type{}); else weights(std::true_type{});
+            if (full) block(std::false_type{}); else block(std::true_type{});
             if constexpr (!CODES) {
                 if (odd) {
                     tmem_wait_st();
@@ -523,7 +549,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[tile]);
         }
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&o_done[tile], (nb - 1) & 1, status));
+        if (ok) ok = __all_sync(0xffffffffu, wait(&o_done[tile], (nb - 1) & 1, status));
         if (ok) {
             tc_fence_after();
             const float l = f2_sum(sum), back = CODES ? unit * (1.0f / 4096.0f) : 1.0f, inv = sh.chunks > 1 ? back : l == 0.f ? 0.f : back / l;
@@ -556,6 +582,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
                 }
                 __syncwarp();                                             // the next load from tensor memory is the whole warp's
             }
+        }
         }
         tc_fence_before();
     }
