@@ -30,9 +30,9 @@ using namespace paged;
 using namespace tc;
 namespace {
 
-constexpr uint32_t ROWS = 128, BP_LOG = 7, BP = 1 << BP_LOG, SLOTS = 4, PANEL = BP * 128;
-constexpr uint32_t SOFTMAX_WARPS = 8, LOAD_WARPS = 4, THREADS = (SOFTMAX_WARPS + LOAD_WARPS + 1) * 32, COLS = 512;
-template <int DIM> constexpr uint32_t tiles_smem() { return 2 * ROWS * DIM * 2 + 4 * BP * DIM * 2 + 1024; }
+constexpr uint32_t ROWS = 128, BP_LOG = 6, BP = 1 << BP_LOG, STAGES = 4, SLOTS = 8, PANEL = BP * 128;
+constexpr uint32_t SOFTMAX_WARPS = 8, LOAD_WARPS = 4, ISSUE_WARP = SOFTMAX_WARPS + LOAD_WARPS, THREADS = (ISSUE_WARP + 2) * 32, COLS = 512;
+template <int DIM> constexpr uint32_t tiles_smem() { return 2 * ROWS * DIM * 2 + 2 * STAGES * BP * DIM * 2 + 1024; }
 
 __device__ __forceinline__ uint32_t claim_columns(uint32_t* slot) {       // by one warp; every other CTA of the SM gives its own back by itself
     tmem_alloc(slot, COLS);
@@ -44,11 +44,20 @@ __device__ __forceinline__ bool elected() {                               // one
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
     return yes != 0;
 }
-// The bounded wait with its loop out of line: what every role goes through stays small (the instruction cache of a scheduler serves four roles).
-__device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity, uint32_t* status) { return mbar_wait_slow<0>(bar, parity, status); }
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, uint32_t* status) { return mbar_try_wait(bar, parity) || wait_on(bar, parity, status); }
-// all loader warps have come here for the n-th time (false: the wait ran out)
-__device__ __forceinline__ bool loaders_meet(uint64_t* bar, uint32_t n, uint32_t lane, uint32_t* status) {
+// The bounded wait (about a second) in few instructions: the instruction cache of a scheduler serves all roles.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, uint32_t* status) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    while (!mbar_try_wait_parked(bar, parity, 2000u)) {
+        if (clock64() - t0 > (1ll << 31)) {
+            atomicOr(status, STATUS_WAIT_TIMEOUT);
+            return false;
+        }
+    }
+    return true;
+}
+// all warps that count on `bar` have come here for the n-th time (false: the wait ran out)
+__device__ __forceinline__ bool warps_meet(uint64_t* bar, uint32_t n, uint32_t lane, uint32_t* status) {
     __syncwarp();
     if (lane == 0) mbar_arrive(bar);
     return __all_sync(0xffffffffu, wait(bar, n & 1, status));
@@ -136,17 +145,17 @@ __device__ __forceinline__ bool find_tile(const Batch& b, uint32_t shift, uint32
 
 template <int DIM, bool CODES, typename Q, typename OUT>
 __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch b, Look look, Shape sh, const Q* q, OUT* out, float* part, float* part_ml, uint32_t* status) {
-    constexpr uint32_t Q_PANEL = ROWS * 128, Q_BYTES = ROWS * DIM * 2, KV_BYTES = BP * DIM * 2, COL_O = 2 * BP;
-    constexpr float ROOM = CODES ? 3.0f : 8.0f;
+    constexpr uint32_t Q_PANEL = ROWS * 128, Q_BYTES = ROWS * DIM * 2, KV_BYTES = BP * DIM * 2, COL_O = 4 * BP;
+    constexpr float MOST = 0x1p11f, UNITS = 16.0f;      // what a block's weights may add up to; a weight is p * v_scale * UNITS / U
     extern __shared__ uint8_t raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    uint8_t *qs = smem, *ks = smem + 2 * Q_BYTES, *vs = ks + 2 * KV_BYTES;
-    // Scales of a block have a barrier per slot.  Slot j % 4 is written next for block j + 4, after K(j + 2) left its place, that is after S(j + 2)
-    // of both tiles, which follows P(j + 1) of every softmax warp.
+    uint8_t *qs = smem, *ks = smem + 2 * Q_BYTES, *vs = ks + STAGES * KV_BYTES;
+    // Scales of a block have a slot and a barrier each.  Slot j % 8 is written next for block j + 8, after K(j + 4) left its place, that is after
+    // S(j + 4), which follows the output of block j + 2 and so every softmax warp's reading of block j.
     __shared__ __align__(16) float s_ks[SLOTS][BP], s_vs[SLOTS][BP];
     __shared__ float s_unit[SLOTS];
-    __shared__ uint32_t s_odd[2];
-    __shared__ uint64_t k_full[2], v_full[2], k_free[2], v_free[2], sc_full[SLOTS], s_full[2], p_full[2], o_done[2], meet;
+    __shared__ uint32_t s_odd[STAGES];
+    __shared__ uint64_t k_full[STAGES], v_full[STAGES], k_free[STAGES], v_free[STAGES], sc_full[SLOTS], s_full[4], p_full[4], o_done[2], o_all[2], meet;      // s, p: tile * 2 + (block & 1)
     __shared__ uint32_t tmem_slot;
     const uint32_t kvh = blockIdx.x % c.kv_heads, chunk = blockIdx.y, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     uint32_t seq = 0, tok0 = 0;
@@ -178,21 +187,26 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
         return;
     }
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2; ++i) {
+        for (uint32_t i = 0; i < STAGES; ++i) {
             mbar_init(&k_full[i], LOAD_WARPS);
             mbar_init(&v_full[i], LOAD_WARPS);
-            mbar_init(&k_free[i], 1);
-            mbar_init(&v_free[i], 1);
+            mbar_init(&k_free[i], tiles);
+            mbar_init(&v_free[i], tiles);
+            s_odd[i] = 0;
+        }
+        for (int i = 0; i < 4; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
+        }
+        for (int i = 0; i < 2; ++i) {
             mbar_init(&o_done[i], 1);
-            s_odd[i] = 0;
+            mbar_init(&o_all[i], 1);
         }
         for (uint32_t i = 0; i < SLOTS; ++i) mbar_init(&sc_full[i], LOAD_WARPS);
         mbar_init(&meet, LOAD_WARPS);
         mbar_fence_init();
     }
-    if (warp == SOFTMAX_WARPS + LOAD_WARPS) claim_columns(&tmem_slot);
+    if (warp == ISSUE_WARP) claim_columns(&tmem_slot);
     // Q: two tiles of 128 rows in 16 bits; a negative scale is taken over by q, so that the largest product is the largest score
     bool clipped = false;
     for (uint32_t i = threadIdx.x; i < 2 * ROWS * (DIM / 8); i += THREADS) {
@@ -217,111 +231,135 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
     const uint32_t tmem = tmem_slot;
     const float scale = fabsf(look.scale);
 
-    if (warp >= SOFTMAX_WARPS && warp < SOFTMAX_WARPS + LOAD_WARPS) {
+    if (warp >= SOFTMAX_WARPS && warp < ISSUE_WARP) {
         constexpr uint32_t CH = CODES ? DIM / 16 : DIM / 8, RP = LOAD_WARPS * 32 / CH, NP = BP / RP;      // 16-byte chunks of a row; rows of a pass; passes
         constexpr uint32_t ROW = DIM * (CODES ? 1 : 2);
         const uint32_t tid = threadIdx.x - SOFTMAX_WARPS * 32, ch = tid % CH, row0 = tid / CH, last16 = last & ~15u;
         bool bad = false, ok = true;
-        // lane g holds where positions 16 g .. 16 g + 15 of a block lie, in sixteens of rows; positions past the last one repeat the last sixteen
-        auto places = [&](uint32_t j) {
-            const uint32_t p = min((blocks.at(lo + j) << BP_LOG) + 16 * (lane & 7), last16);
+        // Where eight blocks lie: lane 4 i + g has positions 16 g .. 16 g + 15 of block 8 m + i, in sixteens of rows (the last sixteen again past
+        // the last position).  The eight blocks behind are asked for as these come into use.
+        constexpr uint32_t G = BP / 16;
+        auto places = [&](uint32_t m) {
+            const uint32_t j = m * (32 / G) + lane / G, p = min((blocks.at(lo + min(j, nb - 1)) << BP_LOG) + 16 * (lane % G), last16);
             return static_cast<uint32_t>(c.row(page_of(c, b, seq, p, bad), kvh, p & (c.size() - 1)) >> 4);
         };
-        auto group = [&](uint32_t i) { return RP <= 16 ? RP * i >> 4 : (RP * i + row0) >> 4; };
-        auto place = [&](const void* array, uint32_t at16, uint32_t i, uint32_t row_bytes) {      // this thread's chunk of pass i
-            return static_cast<const uint8_t*>(array) + static_cast<uint64_t>(__shfl_sync(0xffffffffu, at16, group(i))) * (16 * row_bytes) + ((RP * i + row0) & 15) * row_bytes + 16 * ch;
+        uint32_t here = places(0), there = places(1);
+        auto reach_block = [&](uint32_t j) {                              // (blocks are taken in order)
+            if (j % (32 / G) == 0 && j) { here = there; there = places(j / (32 / G) + 1); }
         };
-        uint32_t here = places(0), there = nb > 1 ? places(1) : here;
+        auto group = [&](uint32_t i) { return RP <= 16 ? RP * i >> 4 : (RP * i + row0) >> 4; };
+        auto place = [&](const void* array, uint32_t j, uint32_t i, uint32_t row_bytes) {         // this thread's chunk of pass i of block j
+            return static_cast<const uint8_t*>(array) + static_cast<uint64_t>(__shfl_sync(0xffffffffu, here, (j * G & 31) + group(i))) * (16 * row_bytes) + ((RP * i + row0) & 15) * row_bytes +
+                   16 * ch;
+        };
         if constexpr (CODES) {
-            uint4 kq[NP], vq[NP];
-            // every warp holds the scales of the whole block, four positions a lane, for the largest of V's; a quarter of the lanes stores
-            float4 k4, v4;
+            // Two blocks ahead, a set of registers for even and one for odd blocks.  Every warp holds the scales of the whole block, two positions a
+            // lane, for the largest of V's; a quarter of the lanes stores.
+            uint4 kq[2][NP], vq[2][NP];
+            float2 k_sc[2], v_sc[2];
             float unit = 0x1p-100f;
-            auto scales = [&](uint32_t at16) {
-                const uint64_t r = static_cast<uint64_t>(__shfl_sync(0xffffffffu, at16, lane >> 2)) * 16 + (4 * lane & 15);
-                k4 = __ldcg(reinterpret_cast<const float4*>(c.k_scale + r));
-                v4 = __ldcg(reinterpret_cast<const float4*>(c.v_scale + r));
+            auto load = [&](const void* from, uint32_t j, uint4 (&x)[NP]) {
+#pragma unroll
+                for (uint32_t i = 0; i < NP; ++i) x[i] = __ldcg(reinterpret_cast<const uint4*>(place(from, j, i, ROW)));
             };
-            auto load = [&](const void* from, uint32_t at16, uint4 (&x)[NP]) {
-#pragma unroll
-                for (uint32_t i = 0; i < NP; ++i) x[i] = __ldcg(reinterpret_cast<const uint4*>(place(from, at16, i, ROW)));
+            auto scales = [&](uint32_t j, uint32_t u) {
+                const uint64_t r = static_cast<uint64_t>(__shfl_sync(0xffffffffu, here, (j * G & 31) + (lane >> 3))) * 16 + (2 * lane & 15);
+                k_sc[u] = __ldcg(reinterpret_cast<const float2*>(c.k_scale + r));
+                v_sc[u] = __ldcg(reinterpret_cast<const float2*>(c.v_scale + r));
             };
-            uint32_t p0 = blocks.at(lo) << BP_LOG;
-            load(c.k, here, kq);
-            scales(here);
-            load(c.v, here, vq);
-            for (uint32_t j = 0; j < nb; ++j) {
-                const uint32_t st = j & 1, par = ((j >> 1) - 1) & 1, slot = j % SLOTS;
-                const uint32_t p1 = j + 1 < nb ? blocks.at(lo + j + 1) << BP_LOG : 0;
-                if (j >= 2) ok = wait(&k_free[st], par, status);
-                if (!__all_sync(0xffffffffu, ok)) break;
 #pragma unroll
-                for (uint32_t i = 0; i < NP; ++i) store_codes(ks + st * KV_BYTES, RP * i + row0, ch, kq[i]);
-                const float vv[4] = {fabsf(v4.x), fabsf(v4.y), fabsf(v4.z), fabsf(v4.w)};
-                float top = 0.f;
+            for (uint32_t u = 0; u < 2; ++u) {
+                if (u < nb) {
+                    load(c.k, u, kq[u]);
+                    scales(u, u);
+                    load(c.v, u, vq[u]);
+                }
+            }
+#pragma unroll 1
+            for (uint32_t j0 = 0; j0 < nb && ok; j0 += 2) {
 #pragma unroll
-                for (uint32_t x = 0; x < 4; ++x)
-                    if (vv[x] < CUDART_INF_F && some_see(look, first, last, p0 + 4 * lane + x)) top = fmaxf(top, vv[x]);
-                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                unit = fmaxf(unit, unit_above(top));
-                if (lane >> 3 == (warp & 3)) {
-                    const float f = 4096.0f / unit;
-                    *reinterpret_cast<float4*>(&s_ks[slot][4 * lane]) = make_float4(k4.x * scale, k4.y * scale, k4.z * scale, k4.w * scale);
-                    *reinterpret_cast<float4*>(&s_vs[slot][4 * lane]) = make_float4(v4.x * f, v4.y * f, v4.z * f, v4.w * f);
-                }
-                if (tid == 0) s_unit[slot] = unit;
-                proxy_fence();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&sc_full[slot]);
-                    mbar_arrive(&k_full[st]);
-                }
-                if (j + 1 < nb) {
-                    load(c.k, there, kq);
-                    scales(there);
-                }
-                if (j >= 2) ok = wait(&v_free[st], par, status);
-                if (!__all_sync(0xffffffffu, ok)) break;
+                for (uint32_t u = 0; u < 2; ++u) {
+                    const uint32_t j = j0 + u, st = j % STAGES, par = (j / STAGES - 1) & 1, slot = j % SLOTS;
+                    if (j >= nb || !ok) break;
+                    const uint32_t p0 = blocks.at(lo + j) << BP_LOG;
+                    const bool more = j + 2 < nb;
+                    if (j >= STAGES) ok = wait(&k_free[st], par, status);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
 #pragma unroll
-                for (uint32_t i = 0; i < NP; ++i) store_codes(vs + st * KV_BYTES, RP * i + row0, ch, vq[i]);
-                proxy_fence();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&v_full[st]);
-                if (j + 1 < nb) {
-                    load(c.v, there, vq);
-                    p0 = p1;
-                    if (j + 2 < nb) there = places(j + 2);
+                    for (uint32_t i = 0; i < NP; ++i) store_codes(ks + st * KV_BYTES, RP * i + row0, ch, kq[u][i]);
+                    const bool all = all_see(look, first, last, p0, BP);
+                    float top = 0.f;
+                    if (fabsf(v_sc[u].x) < CUDART_INF_F && (all || some_see(look, first, last, p0 + 2 * lane))) top = fabsf(v_sc[u].x);
+                    if (fabsf(v_sc[u].y) < CUDART_INF_F && (all || some_see(look, first, last, p0 + 2 * lane + 1))) top = fmaxf(top, fabsf(v_sc[u].y));
+                    unit = fmaxf(unit, unit_above(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)))));       // (of numbers >= 0 the order is that of their bits)
+                    if (lane >> 3 == (warp & 3)) {
+                        const float f = UNITS / unit;
+                        *reinterpret_cast<float2*>(&s_ks[slot][2 * lane]) = make_float2(k_sc[u].x * scale, k_sc[u].y * scale);
+                        *reinterpret_cast<float2*>(&s_vs[slot][2 * lane]) = make_float2(v_sc[u].x * f, v_sc[u].y * f);
+                    }
+                    if (tid == 0) s_unit[slot] = unit;
+                    proxy_fence();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(&sc_full[slot]);
+                        mbar_arrive(&k_full[st]);
+                    }
+                    if (more) {
+                        reach_block(j + 2);
+                        load(c.k, j + 2, kq[u]);
+                        scales(j + 2, u);
+                    }
+                    if (j >= STAGES) ok = wait(&v_free[st], par, status);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+#pragma unroll
+                    for (uint32_t i = 0; i < NP; ++i) store_codes(vs + st * KV_BYTES, RP * i + row0, ch, vq[u][i]);
+                    proxy_fence();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&v_full[st]);
+                    if (more) load(c.v, j + 2, vq[u]);
                 }
             }
         } else {
             const uint32_t to0 = chunk_at(row0, ch, PANEL);                  // (a pass is 8 rows or a multiple: the swizzle of a thread's chunk stays)
-            auto copy = [&](const void* from, uint8_t* to, uint32_t at16, uint32_t p0, bool zeros) {
+            auto copy = [&](const void* from, uint8_t* to, uint32_t j, uint32_t p0, bool zeros) {
                 const uint32_t dst = smem_u32(to) + to0;
 #pragma unroll
                 for (uint32_t i = 0; i < NP; ++i) {
                     const bool take = !zeros || some_see(look, first, last, p0 + RP * i + row0);      // (values that nobody sees are zeros)
-                    copy16(dst + RP * i * 128, place(from, at16, i, ROW), take ? 16 : 0);
+                    copy16(dst + RP * i * 128, place(from, j, i, ROW), take ? 16 : 0);
                 }
                 copies_close();
             };
-            uint32_t p0 = blocks.at(lo) << BP_LOG;
-            copy(c.k, ks, here, p0, false);
-            copy(c.v, vs, here, p0, !all_see(look, first, last, p0, BP));
             uint32_t met = 0;
-            for (uint32_t j = 0; j < nb; ++j) {
-                const uint32_t st = j & 1, other = st ^ 1, par = ((j + 1) >> 1) - 1 & 1;
-                const bool more = j + 1 < nb;
-                const uint32_t p1 = more ? blocks.at(lo + j + 1) << BP_LOG : 0;
-                if (more) {
-                    if (j >= 1) ok = wait(&k_free[other], par, status);
-                    if (!__all_sync(0xffffffffu, ok)) break;
-                    copy(c.k, ks + other * KV_BYTES, there, p1, false);
-                    copies_wait<2>();
-                } else copies_wait<1>();
+            auto bring = [&](uint32_t j) {                                   // block j, keys and values in a group each
+                const uint32_t st = j % STAGES, par = (j / STAGES - 1) & 1, p0 = blocks.at(lo + j) << BP_LOG;
+                reach_block(j);
+                if (j >= STAGES) ok = wait(&k_free[st], par, status);
+                if (!__all_sync(0xffffffffu, ok)) return;
+                copy(c.k, ks + st * KV_BYTES, j, p0, false);
+                if (j >= STAGES) ok = wait(&v_free[st], par, status);
+                if (!__all_sync(0xffffffffu, ok)) return;
+                copy(c.v, vs + st * KV_BYTES, j, p0, !all_see(look, first, last, p0, BP));
+            };
+            bring(0);
+            if (nb > 1) bring(1);
+            for (uint32_t j = 0; j < nb && ok; ++j) {
+                const uint32_t st = j % STAGES, p0 = blocks.at(lo + j) << BP_LOG;
+                if (j + 2 < nb) {
+                    bring(j + 2);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    copies_wait<5>();
+                } else if (j + 1 < nb) copies_wait<3>();
+                else copies_wait<1>();
                 proxy_fence();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&k_full[st]);
-                if (more) copies_wait<1>(); else copies_wait<0>();
+                if (j + 2 < nb) copies_wait<4>();
+                else if (j + 1 < nb) copies_wait<2>();
+                else copies_wait<0>();
                 if (!all_see(look, first, last, p0, BP) && (first != last)) {
                     bool odd = false;
 #pragma unroll
@@ -329,11 +367,11 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
                         const uint4 w = *reinterpret_cast<const uint4*>(vs + st * KV_BYTES + chunk_at(RP * i + row0, ch, PANEL));
                         odd |= holds_nonfinite(w.x) || holds_nonfinite(w.y) || holds_nonfinite(w.z) || holds_nonfinite(w.w);
                     }
-                    // (s_odd of block j - 2 has been read: its V left this place.)  The loaders agree, and then none keeps its part.
+                    // (s_odd of the block before in this place has been read: its V left.)  The loaders agree, and then none keeps its part.
                     if (tid == 0) s_odd[st] = 0;
-                    ok = loaders_meet(&meet, met++, lane, status);
+                    ok = warps_meet(&meet, met++, lane, status);
                     if (odd) s_odd[st] = 1;
-                    ok = ok && loaders_meet(&meet, met++, lane, status);
+                    ok = ok && warps_meet(&meet, met++, lane, status);
                     if (!ok) break;
                     if (*static_cast<volatile uint32_t*>(&s_odd[st]))
 #pragma unroll
@@ -342,64 +380,56 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
                 proxy_fence();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&v_full[st]);
-                if (more) {
-                    if (j >= 1) ok = wait(&v_free[other], par, status);
-                    if (!__all_sync(0xffffffffu, ok)) break;
-                    copy(c.v, vs + other * KV_BYTES, there, p1, !all_see(look, first, last, p1, BP));
-                    p0 = p1;
-                    if (j + 2 < nb) there = places(j + 2);
-                }
             }
             copies_wait<0>();
         }
         if (bad) atomicOr(status, STATUS_BAD_PAGE);
-    } else if (warp >= SOFTMAX_WARPS + LOAD_WARPS) {
-        if (warp == SOFTMAX_WARPS + LOAD_WARPS) {
-            // D f32; A and B f16 or bf16; M = 128; S: both K-major, N = 128; O: B MN-major, N = dim.  The whole warp goes through the waits, so that
-            // addresses and descriptors stay in uniform registers; one lane issues.
-            constexpr uint32_t ID = (1u << 4) | (CODES ? 0u : (1u << 7) | (1u << 10)) | ((ROWS >> 4) << 24), ID_S = ID | ((BP >> 3) << 17), ID_O = ID | (1u << 16) | ((DIM >> 3) << 17);
-            const uint32_t n = __shfl_sync(0xffffffffu, nb, 0), nt = __shfl_sync(0xffffffffu, tiles, 0), base = __shfl_sync(0xffffffffu, tmem, 0);
-            const uint64_t q_desc = smem_desc_sw128(smem_u32(qs)), k_desc = smem_desc_sw128(smem_u32(ks)), v_desc = smem_desc_mn_sw128(smem_u32(vs), PANEL);
-            bool ok = true;
-            // (one place in the code for each product: S(j) of a tile behind its O += P(j - 1) V)
-            for (uint32_t j = 0; j <= n && ok; ++j) {
-                const uint32_t st = j & 1, was = st ^ 1;
-                for (uint32_t t = 0; t < nt && ok; ++t) {
-                    if (j) {
-                        if (t == 0) ok = wait(&v_full[was], ((j - 1) >> 1) & 1, status);
-                        if (ok) ok = wait(&p_full[t], (j - 1) & 1, status);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
-                        tc_fence_after();
-                        if (elected()) {
-                            const uint64_t vd = v_desc + was * (KV_BYTES >> 4);
-#pragma unroll
-                            for (uint32_t kk = 0; kk < BP / 16; ++kk) umma_ts(base + COL_O + t * DIM, base + t * BP + 8 * kk, vd + kk * (16 * 128 >> 4), ID_O, 1u);
-                            tc_commit(&o_done[t]);
-                            if (t + 1 == nt) tc_commit(&v_free[was]);
-                        }
-                        __syncwarp();
-                    }
-                    if (j == n) continue;
-                    if (t == 0) ok = wait(&k_full[st], (j >> 1) & 1, status);
-                    if (ok && j) ok = wait(&o_done[t], (j - 1) & 1, status);                  // P(j - 1) is read: S(j) takes its place
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (elected()) {
-                        const uint64_t qd = q_desc + t * (Q_BYTES >> 4), kd = k_desc + st * (KV_BYTES >> 4);
-#pragma unroll
-                        for (uint32_t kk = 0; kk < DIM / 16; ++kk)
-                            umma_ss(base + t * BP, qd + (kk >> 2) * (Q_PANEL >> 4) + 2 * (kk & 3), kd + (kk >> 2) * (PANEL >> 4) + 2 * (kk & 3), ID_S, kk ? 1u : 0u);
-                        tc_commit(&s_full[t]);
-                        if (t + 1 == nt) tc_commit(&k_free[st]);
-                    }
-                    __syncwarp();
+    } else if (warp >= ISSUE_WARP) {
+        // A warp for each tile.  D f32; A and B f16 or bf16; M = 128; S: both K-major, N = 64; O: B MN-major, N = dim.  The whole warp goes through the
+        // waits, so that addresses and descriptors stay in uniform registers; one lane issues.
+        constexpr uint32_t ID = (1u << 4) | (CODES ? 0u : (1u << 7) | (1u << 10)) | ((ROWS >> 4) << 24), ID_S = ID | ((BP >> 3) << 17), ID_O = ID | (1u << 16) | ((DIM >> 3) << 17);
+        const uint32_t t = warp - ISSUE_WARP, n = t < __shfl_sync(0xffffffffu, tiles, 0) ? __shfl_sync(0xffffffffu, nb, 0) : 0, base = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint64_t q_desc = smem_desc_sw128(smem_u32(qs)) + t * (Q_BYTES >> 4), k_desc = smem_desc_sw128(smem_u32(ks)), v_desc = smem_desc_mn_sw128(smem_u32(vs), PANEL);
+        const bool leader = elected();
+        bool ok = true;
+        // S(j), then O += P(j - 1) V: the next scores are ready when the softmax of this block ends
+#pragma unroll 1
+        for (uint32_t j = 0; n && j <= n; ++j) {
+            const uint32_t st = j % STAGES, was = (j - 1) % STAGES;
+            if (j < n) {
+                if (j >= 2) {                                             // P(j - 2) is read: S(j) takes its place; and the values' place is free
+                    ok = wait(&o_done[t], j & 1, status);
+                    if (leader && ok) mbar_arrive(&v_free[(j - 2) % STAGES]);         // (the loader may want it before it says that K(j) is there)
                 }
+                if (ok) ok = wait(&k_full[st], (j / STAGES) & 1, status);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                tc_fence_after();
+                if (leader) {
+                    const uint64_t kd = k_desc + st * (KV_BYTES >> 4);
+                    const uint32_t d = base + (2 * t + (j & 1)) * BP;
+#pragma unroll
+                    for (uint32_t kk = 0; kk < DIM / 16; ++kk)
+                        umma_ss(d, q_desc + (kk >> 2) * (Q_PANEL >> 4) + 2 * (kk & 3), kd + (kk >> 2) * (PANEL >> 4) + 2 * (kk & 3), ID_S, kk ? 1u : 0u);
+                    tc_commit(&s_full[2 * t + (j & 1)]);
+                }
+                __syncwarp();
             }
+            if (j == 0) continue;
+            ok = wait(&v_full[was], ((j - 1) / STAGES) & 1, status);
+            if (ok) ok = wait(&p_full[2 * t + ((j - 1) & 1)], ((j - 1) >> 1) & 1, status);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            tc_fence_after();
+            if (leader) {
+                const uint64_t vd = v_desc + was * (KV_BYTES >> 4);
+                const uint32_t p = base + (2 * t + ((j - 1) & 1)) * BP;
+#pragma unroll
+                for (uint32_t kk = 0; kk < BP / 16; ++kk) umma_ts(base + COL_O + t * DIM, p + 8 * kk, vd + kk * (16 * 128 >> 4), ID_O, 1u);
+                tc_commit(j == n ? &o_all[t] : &o_done[t]);               // (the last output has a barrier to itself: who waits for it may come late)
+            }
+            __syncwarp();
         }
-    } else {
-        const uint32_t tile = warp / 4, row = threadIdx.x & 127, at = tmem + (((warp & 3) * 32u) << 16), at_s = at + tile * BP, at_o = at + COL_O + tile * DIM;
+    } else if (warp / 4 < tiles) {
+        const uint32_t tile = warp / 4, row = threadIdx.x & 127, at = tmem + (((warp & 3) * 32u) << 16), at_o = at + COL_O + tile * DIM;
         const uint32_t in_tile = row / sh.group, tile_tok = tok0 + tile * sh.tokens, tile_end = min(tile_tok + sh.tokens, end_tok), tok = tile_tok + in_tile;
         const bool live = in_tile < sh.tokens && tok < end_tok, held = live && tok >= lost;
         const uint32_t seen = before + max(min(tok, tile_end - 1), lost);          // (rows that are not there compute on zeros and are not stored)
@@ -407,9 +437,26 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
         // the row sees positions from `low` on, `reach` more, and those below `firsts`
         const uint32_t low = !held ? 1u << 31 : look.window && seen >= look.window ? seen - look.window + 1 : 0, reach = held ? seen - low : 0;
         const uint32_t firsts = held && look.window ? min(look.sinks, seen + 1) : 0;
-        float mx = -CUDART_INF_F, unit = 0x1p-100f;
+        const auto sees = [&](uint32_t p) { return static_cast<bool>((p - low <= reach) | (p < firsts)); };
+        float mx = held ? -CUDART_INF_F : 0.f, unit = 0x1p-100f;          // (a row that sees nothing needs no maximum)
         f2 sum = 0;
         bool ok = true;
+        const f2 sc2 = f2_both(scale);
+        auto scale_output = [&](uint32_t j, float corr) {                 // what blocks before j gave
+            ok = ok && __all_sync(0xffffffffu, wait(&o_done[tile], (j - 1) & 1, status));
+            if (!ok) return;
+            tc_fence_after();
+#pragma unroll 1
+            for (uint32_t col = 0; col < DIM; col += 16) {
+                uint32_t o[16];
+                tmem_ld16(at_o + col, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                tmem_st16(at_o + col, o);
+            }
+            tmem_wait_st();
+        };
         {
             uint32_t zero[32];
 #pragma unroll
@@ -417,106 +464,138 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
 #pragma unroll
             for (uint32_t col = 0; col < DIM; col += 32) tmem_st32(at_o + col, zero);
         }
-        if (tile < tiles) {
+#pragma unroll 1
         for (uint32_t j = 0; j < nb; ++j) {
-            const uint32_t slot = j % SLOTS, st = j & 1, p0 = blocks.at(lo + j) << BP_LOG;
-            ok = wait(&s_full[tile], j & 1, status);
-            if constexpr (CODES) { if (ok) ok = wait(&sc_full[slot], (j / SLOTS) & 1, status); }
+            const uint32_t slot = j % SLOTS, st = j % STAGES, p0 = blocks.at(lo + j) << BP_LOG, at_s = at + (2 * tile + (j & 1)) * BP;
             const bool full = all_see(look, t_first, t_last, p0, BP) && tile_tok >= lost;
+            ok = wait(&s_full[2 * tile + (j & 1)], (j >> 1) & 1, status);
+            if constexpr (CODES) { if (ok) ok = wait(&sc_full[slot], (j / SLOTS) & 1, status); }
             bool odd = false;
             if constexpr (!CODES) {
                 if (!all_see(look, first, last, p0, BP) && first != last) {
-                    if (ok) ok = wait(&v_full[st], (j >> 1) & 1, status);
+                    if (ok) ok = wait(&v_full[st], (j / STAGES) & 1, status);
                     odd = *static_cast<volatile uint32_t*>(&s_odd[st]) != 0;
                 }
             }
-            ok = __all_sync(0xffffffffu, ok);
+            if (ok && row == 0) mbar_arrive(&k_free[st]);                 // the scores are there: the keys' place is free
+            ok = __all_sync(0xffffffffu, ok);                             // (and the warp is together again, as accesses to tensor memory want it)
             if (!ok) break;
             tc_fence_after();
             const ulonglong2 *k2 = reinterpret_cast<const ulonglong2*>(s_ks[slot]), *v2 = reinterpret_cast<const ulonglong2*>(s_vs[slot]);
-            const auto sees = [&](uint32_t p) { return p - low <= reach || p < firsts; };
-            auto block = [&](auto masked) {
-                constexpr bool MASKED = decltype(masked)::value;
-                // twice over the scores, 32 columns at a time: the maximum, then the exponentials
-                float top[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+            if constexpr (CODES) {
+                const float above = s_unit[slot];
+                if (above != unit) {
+                    if (j) scale_output(j, unit / above);
+                    unit = above;
+                }
+            }
+            // weights of 32 columns -> tensor memory, over scores that have been read
+            auto store = [&](uint32_t x, const f2* e, auto masked) {
+                uint32_t p[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float2 w = f2_parts(e[i]);
+                    if constexpr (CODES) {
+                        const ulonglong2 v = v2[8 * x + i / 2];
+                        w = f2_parts(f2_mul(e[i], i & 1 ? v.y : v.x));
+                        if constexpr (decltype(masked)::value) {          // (also where the scale of V is infinite or NaN)
+                            if (!sees(p0 + 32 * x + 2 * i)) w.x = 0.f;
+                            if (!sees(p0 + 32 * x + 2 * i + 1)) w.y = 0.f;
+                        }
+                    }
+                    p[i] = pack2<CODES>(w.x, w.y);
+                }
+                if constexpr (decltype(masked)::value) __syncwarp();
+                tmem_st16(at_s + 16 * x, p);
+            };
+            auto factor = [&](uint32_t x, int i) {
+                if constexpr (!CODES) return sc2;
+                const ulonglong2 k = k2[8 * x + i / 2];
+                return static_cast<f2>(i & 1 ? k.y : k.x);
+            };
+            if (full && !__any_sync(0xffffffffu, mx == -CUDART_INF_F)) {
+                // All rows have a maximum of earlier blocks: weights are taken against that, in one pass, and as long as they add up to no more
+                // than MOST it stays (what they add up to is at least the largest of them).
+                f2 e[BP / 2], part;
+                for (bool again = false;; again = true) {
+                    uint32_t r[2][32];
+                    tmem_ld32(at_s, r[0]);
+                    tmem_ld32(at_s + 32, r[1]);
+                    tmem_wait_ld();
+                    const f2 nm = f2_both(-mx);
+                    f2 s0 = 0, s1 = 0;
+#pragma unroll
+                    for (int i = 0; i < static_cast<int>(BP / 2); ++i) {
+                        const float2 d = f2_parts(f2_fma(f2_of(__uint_as_float(r[i / 16][2 * (i % 16)]), __uint_as_float(r[i / 16][2 * (i % 16) + 1])), factor(i / 16, i % 16), nm));
+                        e[i] = f2_of(ex2(d.x), ex2(d.y));
+                        if (i & 1) s1 = f2_add(s1, e[i]); else s0 = f2_add(s0, e[i]);
+                    }
+                    part = f2_add(s0, s1);
+                    if (again || !__any_sync(0xffffffffu, f2_sum(part) > MOST)) break;
+                    // a new maximum: output and sums so far follow
+                    float top = 0.f;
+#pragma unroll 1
+                    for (uint32_t x = 0; x < BP / 32; ++x) {
+                        tmem_ld32(at_s + 32 * x, r[0]);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float2 d = f2_parts(f2_fma(f2_of(__uint_as_float(r[0][2 * i]), __uint_as_float(r[0][2 * i + 1])), factor(x, i), nm));
+                            top = fmaxf(top, fmaxf(d.x, d.y));
+                        }
+                    }
+                    const float corr = ex2(-top);
+                    mx += top;
+                    sum = f2_mul(sum, f2_both(corr));
+                    scale_output(j, corr);                                // (there is a block before: it gave the maximum)
+                }
+                sum = f2_add(sum, part);
+                store(0, e, std::false_type{});
+                store(1, e + 16, std::false_type{});
+            } else {
+                // masks, or the first block that a row sees: twice over the scores
+                float top = -CUDART_INF_F;
+                auto score = [&](uint32_t x, int i, const uint32_t (&r)[32]) {
+                    float2 v = f2_parts(f2_mul(f2_of(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), factor(x, i)));
+                    if (!sees(p0 + 32 * x + 2 * i)) v.x = -CUDART_INF_F;
+                    if (!sees(p0 + 32 * x + 2 * i + 1)) v.y = -CUDART_INF_F;
+                    return v;
+                };
 #pragma unroll 1
                 for (uint32_t x = 0; x < BP / 32; ++x) {
                     uint32_t r[32];
                     tmem_ld32(at_s + 32 * x, r);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        float2 v = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-                        if constexpr (CODES) { const ulonglong2 k = k2[8 * x + i / 2]; v = f2_parts(f2_mul(f2_of(v.x, v.y), i & 1 ? k.y : k.x)); }
-                        if constexpr (MASKED) {
-                            if (!sees(p0 + 32 * x + 2 * i)) v.x = -CUDART_INF_F;
-                            if (!sees(p0 + 32 * x + 2 * i + 1)) v.y = -CUDART_INF_F;
-                        }
-                        top[i & 3] = fmaxf(fmaxf(top[i & 3], v.x), v.y);
-                    }
+                    for (int i = 0; i < 16; ++i) { const float2 v = score(x, i, r); top = fmaxf(top, fmaxf(v.x, v.y)); }
+                    __syncwarp();
                 }
-                float bm = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                if constexpr (!CODES) bm = bm == -CUDART_INF_F ? bm : bm * scale;
-                // the output is in units of `unit` times exp2 of the maximum
-                const float above = CODES ? s_unit[slot] : unit;
-                const bool grew = bm > mx + ROOM || (mx == -CUDART_INF_F && bm > mx);
-                if (__any_sync(0xffffffffu, grew || above != unit)) {
-                    const float to = grew ? bm : mx;
-                    float corr = grew ? ex2(mx - to) : 1.0f;
+                const bool grew = top > mx;
+                if (__any_sync(0xffffffffu, grew)) {
+                    const float to = grew ? top : mx, corr = grew ? ex2(mx - to) : 1.0f;
                     sum = f2_mul(sum, f2_both(corr));
                     mx = to;
-                    corr *= unit / above;
-                    unit = above;
-                    if (j) {                                              // (S(j) followed the output of block j - 1)
-#pragma unroll 1
-                        for (uint32_t col = 0; col < DIM; col += 16) {
-                            uint32_t o[16];
-                            tmem_ld16(at_o + col, o);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-                            tmem_st16(at_o + col, o);
-                        }
-                    }
+                    if (j) scale_output(j, corr);
                 }
-                const f2 nm = f2_both(mx == -CUDART_INF_F ? 0.f : -mx), sc2 = f2_both(scale);
+                const float zero = mx == -CUDART_INF_F ? 0.f : mx;
 #pragma unroll 1
                 for (uint32_t x = 0; x < BP / 32; ++x) {
-                    uint32_t r[32], p[16];
+                    uint32_t r[32];
                     tmem_ld32(at_s + 32 * x, r);
                     tmem_wait_ld();
+                    f2 e[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        f2 k = sc2;
-                        if constexpr (CODES) { const ulonglong2 kk = k2[8 * x + i / 2]; k = i & 1 ? kk.y : kk.x; }
-                        float2 d = f2_parts(f2_fma(f2_of(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), k, nm));
-                        bool s0 = true, s1 = true;
-                        if constexpr (MASKED) {
-                            s0 = sees(p0 + 32 * x + 2 * i);
-                            s1 = sees(p0 + 32 * x + 2 * i + 1);
-                            if (!s0) d.x = -CUDART_INF_F;
-                            if (!s1) d.y = -CUDART_INF_F;
-                        }
-                        const f2 e = f2_of(ex2(d.x), ex2(d.y));
-                        sum = f2_add(sum, e);
-                        float2 w = f2_parts(e);
-                        if constexpr (CODES) {
-                            const ulonglong2 v = v2[8 * x + i / 2];
-                            w = f2_parts(f2_mul(e, i & 1 ? v.y : v.x));
-                            if constexpr (MASKED) {                       // (also where the scale of V is infinite or NaN)
-                                if (!s0) w.x = 0.f;
-                                if (!s1) w.y = 0.f;
-                            }
-                        }
-                        p[i] = pack2<CODES>(w.x, w.y);
+                        const float2 v = score(x, i, r);
+                        e[i] = f2_of(ex2(v.x - zero), ex2(v.y - zero));
+                        sum = f2_add(sum, e[i]);
                     }
-                    tmem_st16(at_s + 16 * x, p);                          // over scores that have been read
+                    store(x, e, std::true_type{});
                 }
-            };
-            if (full) block(std::false_type{}); else block(std::true_type{});
+            }
+            tmem_wait_st();
             if constexpr (!CODES) {
                 if (odd) {
-                    tmem_wait_st();
 #pragma unroll 1
                     for (uint32_t p16 = 0; p16 < BP / 16; ++p16) {
                         uint32_t w[16];
@@ -544,51 +623,51 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
                     }
                 }
             }
-            tmem_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[tile]);
+            if (lane == 0) mbar_arrive(&p_full[2 * tile + (j & 1)]);
         }
-        if (ok) ok = __all_sync(0xffffffffu, wait(&o_done[tile], (nb - 1) & 1, status));
+        if (ok) ok = wait(&o_all[tile], 0, status);
+        ok = __all_sync(0xffffffffu, ok);
         if (ok) {
             tc_fence_after();
-            const float l = f2_sum(sum), back = CODES ? unit * (1.0f / 4096.0f) : 1.0f, inv = sh.chunks > 1 ? back : l == 0.f ? 0.f : back / l;
+            const float l = f2_sum(sum), back = CODES ? unit * (1.0f / UNITS) : 1.0f, inv = sh.chunks > 1 ? back : l == 0.f ? 0.f : back / l;
             const size_t orow = static_cast<size_t>(span.row0) + (live ? tok : tok0), head = static_cast<size_t>(kvh) * sh.group + (live ? row % sh.group : 0);
             OUT* dst = out + orow * sh.ldo + head * DIM;
             const size_t at_part = (orow * sh.heads + head) * sh.chunks + chunk;
             const bool wide = reinterpret_cast<uintptr_t>(dst) % 16 == 0;
             if (sh.chunks > 1 && live) *reinterpret_cast<float2*>(part_ml + 2 * at_part) = make_float2(mx, l);
+            __syncwarp();
 #pragma unroll 1
-            for (uint32_t col = 0; col < DIM; col += 32) {
-                uint32_t o[32];
-                tmem_ld32(at_o + col, o);
+            for (uint32_t col = 0; col < DIM; col += 16) {
+                uint32_t o[16];
+                tmem_ld16(at_o + col, o);
                 tmem_wait_ld();
                 if (live && sh.chunks > 1) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
+                    for (int i = 0; i < 4; ++i)
                         reinterpret_cast<float4*>(part + at_part * DIM + col)[i] = make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
                                                                                                __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
                 } else if (live) {
-                    __align__(16) OUT h[32];
+                    __align__(16) OUT h[16];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) h[i] = out_value<OUT>(l == 0.f ? 0.f : __uint_as_float(o[i]) * inv, clipped);
+                    for (int i = 0; i < 16; ++i) h[i] = out_value<OUT>(l == 0.f ? 0.f : __uint_as_float(o[i]) * inv, clipped);
                     if (wide) {
 #pragma unroll
-                        for (int i = 0; i < static_cast<int>(2 * sizeof(OUT)); ++i) reinterpret_cast<uint4*>(dst + col)[i] = reinterpret_cast<const uint4*>(h)[i];
+                        for (int i = 0; i < static_cast<int>(sizeof(OUT)); ++i) reinterpret_cast<uint4*>(dst + col)[i] = reinterpret_cast<const uint4*>(h)[i];
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) dst[col + i] = h[i];
+                        for (int i = 0; i < 16; ++i) dst[col + i] = h[i];
                     }
                 }
                 __syncwarp();                                             // the next load from tensor memory is the whole warp's
             }
         }
-        }
         tc_fence_before();
     }
     if (clipped) atomicOr(status, STATUS_X_CLIPPED);
     __syncthreads();
-    if (warp == SOFTMAX_WARPS + LOAD_WARPS) { tc_fence_after(); tmem_dealloc(tmem, COLS); }
+    if (warp == ISSUE_WARP) { tc_fence_after(); tmem_dealloc(tmem, COLS); }
 }
 
 template <int DIM, bool CODES, typename Q, typename OUT>
