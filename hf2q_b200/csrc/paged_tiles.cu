@@ -31,7 +31,13 @@ using namespace tc;
 namespace {
 
 constexpr uint32_t ROWS = 128, BP_LOG = 6, BP = 1 << BP_LOG, STAGES = 4, SLOTS = 8, PANEL = BP * 128;
-constexpr uint32_t SOFTMAX_WARPS = 8, LOAD_WARPS = 4, ISSUE_WARP = SOFTMAX_WARPS + LOAD_WARPS, THREADS = (ISSUE_WARP + 2) * 32, COLS = 512;
+constexpr uint32_t SOFTMAX_WARPS = 8, LOAD_WARPS = 4, ISSUE_WARP = SOFTMAX_WARPS + 2 * LOAD_WARPS, THREADS = (ISSUE_WARP + 4) * 32, COLS = 512;
+// Registers of a thread: 96 at launch; the softmax threads take 48 more, which the loaders and the issuing group of four warps give up (2 x 144 + 2 x 72
+// + 48 = 5 x 96).
+constexpr int SOFTMAX_REGS = 144, LOAD_REGS = 72, ISSUE_REGS = 48;
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+constexpr uint32_t APART = 8;
 template <int DIM> constexpr uint32_t tiles_smem() { return 2 * ROWS * DIM * 2 + 2 * STAGES * BP * DIM * 2 + 1024; }
 
 __device__ __forceinline__ uint32_t claim_columns(uint32_t* slot) {       // by one warp; every other CTA of the SM gives its own back by itself
@@ -155,7 +161,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
     __shared__ __align__(16) float s_ks[SLOTS][BP], s_vs[SLOTS][BP];
     __shared__ float s_unit[SLOTS];
     __shared__ uint32_t s_odd[STAGES];
-    __shared__ uint64_t k_full[STAGES], v_full[STAGES], k_free[STAGES], v_free[STAGES], sc_full[SLOTS], s_full[4], p_full[4], o_done[2], o_all[2], meet;      // s, p: tile * 2 + (block & 1)
+    __shared__ uint64_t k_full[STAGES], v_full[STAGES], k_free[STAGES], v_free[STAGES], sc_full[SLOTS], s_full[4], p_full[4], o_done[2], o_all[2], meet, apart;      // s, p: tile * 2 + (block & 1)
     __shared__ uint32_t tmem_slot;
     const uint32_t kvh = blockIdx.x % c.kv_heads, chunk = blockIdx.y, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     uint32_t seq = 0, tok0 = 0;
@@ -202,8 +208,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
             mbar_init(&o_done[i], 1);
             mbar_init(&o_all[i], 1);
         }
-        for (uint32_t i = 0; i < SLOTS; ++i) mbar_init(&sc_full[i], LOAD_WARPS);
+        for (uint32_t i = 0; i < SLOTS; ++i) mbar_init(&sc_full[i], 2 * LOAD_WARPS);
         mbar_init(&meet, LOAD_WARPS);
+        mbar_init(&apart, 1);
         mbar_fence_init();
     }
     if (warp == ISSUE_WARP) claim_columns(&tmem_slot);
@@ -232,13 +239,17 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
     const float scale = fabsf(look.scale);
 
     if (warp >= SOFTMAX_WARPS && warp < ISSUE_WARP) {
+        // Four warps for the keys, four for the values.
+        fewer_registers<LOAD_REGS>();
         constexpr uint32_t CH = CODES ? DIM / 16 : DIM / 8, RP = LOAD_WARPS * 32 / CH, NP = BP / RP;      // 16-byte chunks of a row; rows of a pass; passes
-        constexpr uint32_t ROW = DIM * (CODES ? 1 : 2);
-        const uint32_t tid = threadIdx.x - SOFTMAX_WARPS * 32, ch = tid % CH, row0 = tid / CH, last16 = last & ~15u;
+        constexpr uint32_t ROW = DIM * (CODES ? 1 : 2), G = BP / 16;
+        const bool keys = warp < SOFTMAX_WARPS + LOAD_WARPS;
+        const uint32_t tid = threadIdx.x & 127, ch = tid % CH, row0 = tid / CH, last16 = last & ~15u;
+        uint8_t* stages = keys ? ks : vs;
+        uint64_t *full_bars = keys ? k_full : v_full, *free_bars = keys ? k_free : v_free;
         bool bad = false, ok = true;
         // Where eight blocks lie: lane 4 i + g has positions 16 g .. 16 g + 15 of block 8 m + i, in sixteens of rows (the last sixteen again past
         // the last position).  The eight blocks behind are asked for as these come into use.
-        constexpr uint32_t G = BP / 16;
         auto places = [&](uint32_t m) {
             const uint32_t j = m * (32 / G) + lane / G, p = min((blocks.at(lo + min(j, nb - 1)) << BP_LOG) + 16 * (lane % G), last16);
             return static_cast<uint32_t>(c.row(page_of(c, b, seq, p, bad), kvh, p & (c.size() - 1)) >> 4);
@@ -247,124 +258,95 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
         auto reach_block = [&](uint32_t j) {                              // (blocks are taken in order)
             if (j % (32 / G) == 0 && j) { here = there; there = places(j / (32 / G) + 1); }
         };
-        auto group = [&](uint32_t i) { return RP <= 16 ? RP * i >> 4 : (RP * i + row0) >> 4; };
-        auto place = [&](const void* array, uint32_t j, uint32_t i, uint32_t row_bytes) {         // this thread's chunk of pass i of block j
-            return static_cast<const uint8_t*>(array) + static_cast<uint64_t>(__shfl_sync(0xffffffffu, here, (j * G & 31) + group(i))) * (16 * row_bytes) + ((RP * i + row0) & 15) * row_bytes +
-                   16 * ch;
+        const uint8_t* mine = static_cast<const uint8_t*>(keys ? c.k : c.v) + (row0 & 15) * ROW + 16 * ch;
+        auto place = [&](uint32_t j, uint32_t i) {                        // this thread's chunk of pass i of block j
+            const uint32_t at16 = __shfl_sync(0xffffffffu, here, (j * G & 31) + (RP <= 16 ? RP * i >> 4 : (RP * i + row0) >> 4));
+            return mine + static_cast<uint64_t>(at16) * (16 * ROW) + (RP * i & 15) * ROW;
         };
         if constexpr (CODES) {
             // Two blocks ahead, a set of registers for even and one for odd blocks.  Every warp holds the scales of the whole block, two positions a
             // lane, for the largest of V's; a quarter of the lanes stores.
-            uint4 kq[2][NP], vq[2][NP];
-            float2 k_sc[2], v_sc[2];
+            const float* scales = keys ? c.k_scale : c.v_scale;
+            uint4 x[2][NP];
+            float2 sc[2];
             float unit = 0x1p-100f;
-            auto load = [&](const void* from, uint32_t j, uint4 (&x)[NP]) {
+            auto load = [&](uint32_t j, uint32_t u) {
 #pragma unroll
-                for (uint32_t i = 0; i < NP; ++i) x[i] = __ldcg(reinterpret_cast<const uint4*>(place(from, j, i, ROW)));
+                for (uint32_t i = 0; i < NP; ++i) x[u][i] = __ldcg(reinterpret_cast<const uint4*>(place(j, i)));
+                sc[u] = __ldcg(reinterpret_cast<const float2*>(scales + (static_cast<uint64_t>(__shfl_sync(0xffffffffu, here, (j * G & 31) + (lane >> 3))) * 16 + (2 * lane & 15))));
             };
-            auto scales = [&](uint32_t j, uint32_t u) {
-                const uint64_t r = static_cast<uint64_t>(__shfl_sync(0xffffffffu, here, (j * G & 31) + (lane >> 3))) * 16 + (2 * lane & 15);
-                k_sc[u] = __ldcg(reinterpret_cast<const float2*>(c.k_scale + r));
-                v_sc[u] = __ldcg(reinterpret_cast<const float2*>(c.v_scale + r));
-            };
-#pragma unroll
-            for (uint32_t u = 0; u < 2; ++u) {
-                if (u < nb) {
-                    load(c.k, u, kq[u]);
-                    scales(u, u);
-                    load(c.v, u, vq[u]);
-                }
-            }
+            load(0, 0);
+            if (nb > 1) load(1, 1);
 #pragma unroll 1
             for (uint32_t j0 = 0; j0 < nb && ok; j0 += 2) {
 #pragma unroll
                 for (uint32_t u = 0; u < 2; ++u) {
-                    const uint32_t j = j0 + u, st = j % STAGES, par = (j / STAGES - 1) & 1, slot = j % SLOTS;
+                    const uint32_t j = j0 + u, st = j % STAGES, slot = j % SLOTS;
                     if (j >= nb || !ok) break;
-                    const uint32_t p0 = blocks.at(lo + j) << BP_LOG;
-                    const bool more = j + 2 < nb;
-                    if (j >= STAGES) ok = wait(&k_free[st], par, status);
+                    if (j >= STAGES) ok = wait(&free_bars[st], (j / STAGES - 1) & 1, status);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
 #pragma unroll
-                    for (uint32_t i = 0; i < NP; ++i) store_codes(ks + st * KV_BYTES, RP * i + row0, ch, kq[u][i]);
-                    const bool all = all_see(look, first, last, p0, BP);
-                    float top = 0.f;
-                    if (fabsf(v_sc[u].x) < CUDART_INF_F && (all || some_see(look, first, last, p0 + 2 * lane))) top = fabsf(v_sc[u].x);
-                    if (fabsf(v_sc[u].y) < CUDART_INF_F && (all || some_see(look, first, last, p0 + 2 * lane + 1))) top = fmaxf(top, fabsf(v_sc[u].y));
-                    unit = fmaxf(unit, unit_above(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)))));       // (of numbers >= 0 the order is that of their bits)
-                    if (lane >> 3 == (warp & 3)) {
-                        const float f = UNITS / unit;
-                        *reinterpret_cast<float2*>(&s_ks[slot][2 * lane]) = make_float2(k_sc[u].x * scale, k_sc[u].y * scale);
-                        *reinterpret_cast<float2*>(&s_vs[slot][2 * lane]) = make_float2(v_sc[u].x * f, v_sc[u].y * f);
+                    for (uint32_t i = 0; i < NP; ++i) store_codes(stages + st * KV_BYTES, RP * i + row0, ch, x[u][i]);
+                    float f = scale;
+                    if (!keys) {
+                        const uint32_t p0 = blocks.at(lo + j) << BP_LOG;
+                        const bool all = all_see(look, first, last, p0, BP);
+                        float top = 0.f;
+                        if (fabsf(sc[u].x) < CUDART_INF_F && (all || some_see(look, first, last, p0 + 2 * lane))) top = fabsf(sc[u].x);
+                        if (fabsf(sc[u].y) < CUDART_INF_F && (all || some_see(look, first, last, p0 + 2 * lane + 1))) top = fmaxf(top, fabsf(sc[u].y));
+                        unit = fmaxf(unit, unit_above(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)))));       // (of numbers >= 0 the order is that of their bits)
+                        f = __uint_as_float((258u << 23) - __float_as_uint(unit));          // UNITS / unit, of powers of two
+                        if (tid == 0) s_unit[slot] = unit;
                     }
-                    if (tid == 0) s_unit[slot] = unit;
+                    if (lane >> 3 == (warp & 3)) *reinterpret_cast<float2*>(&(keys ? s_ks : s_vs)[slot][2 * lane]) = make_float2(sc[u].x * f, sc[u].y * f);
                     proxy_fence();
                     __syncwarp();
                     if (lane == 0) {
                         mbar_arrive(&sc_full[slot]);
-                        mbar_arrive(&k_full[st]);
+                        mbar_arrive(&full_bars[st]);
                     }
-                    if (more) {
+                    if (j + 2 < nb) {
                         reach_block(j + 2);
-                        load(c.k, j + 2, kq[u]);
-                        scales(j + 2, u);
+                        load(j + 2, u);
                     }
-                    if (j >= STAGES) ok = wait(&v_free[st], par, status);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-#pragma unroll
-                    for (uint32_t i = 0; i < NP; ++i) store_codes(vs + st * KV_BYTES, RP * i + row0, ch, vq[u][i]);
-                    proxy_fence();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&v_full[st]);
-                    if (more) load(c.v, j + 2, vq[u]);
                 }
             }
         } else {
-            const uint32_t to0 = chunk_at(row0, ch, PANEL);                  // (a pass is 8 rows or a multiple: the swizzle of a thread's chunk stays)
-            auto copy = [&](const void* from, uint8_t* to, uint32_t j, uint32_t p0, bool zeros) {
-                const uint32_t dst = smem_u32(to) + to0;
+            const uint32_t to0 = smem_u32(stages) + chunk_at(row0, ch, PANEL);       // (a pass is 8 rows or a multiple: the swizzle of a thread's chunk stays)
+            uint32_t met = 0;
+            auto bring = [&](uint32_t j) {                                // block j, as a group of copies
+                const uint32_t st = j % STAGES, p0 = blocks.at(lo + j) << BP_LOG, to = to0 + st * KV_BYTES;
+                reach_block(j);
+                if (j >= STAGES) ok = wait(&free_bars[st], (j / STAGES - 1) & 1, status);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) return;
+                if (keys || all_see(look, first, last, p0, BP)) {
 #pragma unroll
-                for (uint32_t i = 0; i < NP; ++i) {
-                    const bool take = !zeros || some_see(look, first, last, p0 + RP * i + row0);      // (values that nobody sees are zeros)
-                    copy16(dst + RP * i * 128, place(from, j, i, ROW), take ? 16 : 0);
+                    for (uint32_t i = 0; i < NP; ++i) copy16(to + RP * i * 128, place(j, i), 16);
+                } else {                                                  // (values that nobody sees are zeros)
+#pragma unroll
+                    for (uint32_t i = 0; i < NP; ++i) copy16(to + RP * i * 128, place(j, i), some_see(look, first, last, p0 + RP * i + row0) ? 16 : 0);
                 }
                 copies_close();
             };
-            uint32_t met = 0;
-            auto bring = [&](uint32_t j) {                                   // block j, keys and values in a group each
-                const uint32_t st = j % STAGES, par = (j / STAGES - 1) & 1, p0 = blocks.at(lo + j) << BP_LOG;
-                reach_block(j);
-                if (j >= STAGES) ok = wait(&k_free[st], par, status);
-                if (!__all_sync(0xffffffffu, ok)) return;
-                copy(c.k, ks + st * KV_BYTES, j, p0, false);
-                if (j >= STAGES) ok = wait(&v_free[st], par, status);
-                if (!__all_sync(0xffffffffu, ok)) return;
-                copy(c.v, vs + st * KV_BYTES, j, p0, !all_see(look, first, last, p0, BP));
-            };
             bring(0);
             if (nb > 1) bring(1);
+#pragma unroll 1
             for (uint32_t j = 0; j < nb && ok; ++j) {
                 const uint32_t st = j % STAGES, p0 = blocks.at(lo + j) << BP_LOG;
                 if (j + 2 < nb) {
                     bring(j + 2);
-                    ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    copies_wait<5>();
-                } else if (j + 1 < nb) copies_wait<3>();
-                else copies_wait<1>();
-                proxy_fence();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&k_full[st]);
-                if (j + 2 < nb) copies_wait<4>();
-                else if (j + 1 < nb) copies_wait<2>();
+                    copies_wait<2>();
+                } else if (j + 1 < nb) copies_wait<1>();
                 else copies_wait<0>();
-                if (!all_see(look, first, last, p0, BP) && (first != last)) {
+                if (!keys && !all_see(look, first, last, p0, BP) && first != last) {
+                    uint8_t* to = stages + st * KV_BYTES + chunk_at(row0, ch, PANEL);
                     bool odd = false;
 #pragma unroll
                     for (uint32_t i = 0; i < NP; ++i) {
-                        const uint4 w = *reinterpret_cast<const uint4*>(vs + st * KV_BYTES + chunk_at(RP * i + row0, ch, PANEL));
+                        const uint4 w = *reinterpret_cast<const uint4*>(to + RP * i * 128);
                         odd |= holds_nonfinite(w.x) || holds_nonfinite(w.y) || holds_nonfinite(w.z) || holds_nonfinite(w.w);
                     }
                     // (s_odd of the block before in this place has been read: its V left.)  The loaders agree, and then none keeps its part.
@@ -375,16 +357,17 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
                     if (!ok) break;
                     if (*static_cast<volatile uint32_t*>(&s_odd[st]))
 #pragma unroll
-                        for (uint32_t i = 0; i < NP; ++i) *reinterpret_cast<uint4*>(vs + st * KV_BYTES + chunk_at(RP * i + row0, ch, PANEL)) = make_uint4(0u, 0u, 0u, 0u);
+                        for (uint32_t i = 0; i < NP; ++i) *reinterpret_cast<uint4*>(to + RP * i * 128) = make_uint4(0u, 0u, 0u, 0u);
                 }
                 proxy_fence();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&v_full[st]);
+                if (lane == 0) mbar_arrive(&full_bars[st]);
             }
             copies_wait<0>();
         }
         if (bad) atomicOr(status, STATUS_BAD_PAGE);
     } else if (warp >= ISSUE_WARP) {
+        fewer_registers<ISSUE_REGS>();
         // A warp for each tile.  D f32; A and B f16 or bf16; M = 128; S: both K-major, N = 64; O: B MN-major, N = dim.  The whole warp goes through the
         // waits, so that addresses and descriptors stay in uniform registers; one lane issues.
         constexpr uint32_t ID = (1u << 4) | (CODES ? 0u : (1u << 7) | (1u << 10)) | ((ROWS >> 4) << 24), ID_S = ID | ((BP >> 3) << 17), ID_O = ID | (1u << 16) | ((DIM >> 3) << 17);
@@ -392,6 +375,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
         const uint64_t q_desc = smem_desc_sw128(smem_u32(qs)) + t * (Q_BYTES >> 4), k_desc = smem_desc_sw128(smem_u32(ks)), v_desc = smem_desc_mn_sw128(smem_u32(vs), PANEL);
         const bool leader = elected();
         bool ok = true;
+        // The second tile starts when the first has its first weights: half a round later, so that one takes exponentials while the other loads, stores
+        // and waits.  (Few blocks end sooner side by side.)
+        if (t == 1 && n >= APART) ok = wait(&apart, 0, status);
         // S(j), then O += P(j - 1) V: the next scores are ready when the softmax of this block ends
 #pragma unroll 1
         for (uint32_t j = 0; n && j <= n; ++j) {
@@ -428,7 +414,8 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
             }
             __syncwarp();
         }
-    } else if (warp / 4 < tiles) {
+    } else {
+        more_registers<SOFTMAX_REGS>();
         const uint32_t tile = warp / 4, row = threadIdx.x & 127, at = tmem + (((warp & 3) * 32u) << 16), at_o = at + COL_O + tile * DIM;
         const uint32_t in_tile = row / sh.group, tile_tok = tok0 + tile * sh.tokens, tile_end = min(tile_tok + sh.tokens, end_tok), tok = tile_tok + in_tile;
         const bool live = in_tile < sh.tokens && tok < end_tok, held = live && tok >= lost;
@@ -438,9 +425,15 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
         const uint32_t low = !held ? 1u << 31 : look.window && seen >= look.window ? seen - look.window + 1 : 0, reach = held ? seen - low : 0;
         const uint32_t firsts = held && look.window ? min(look.sinks, seen + 1) : 0;
         const auto sees = [&](uint32_t p) { return static_cast<bool>((p - low <= reach) | (p < firsts)); };
+        // blocks that start at full0 .. full0 + full_reach are seen whole by every row of the tile (blocks of the first positions beside a window are not
+        // counted here)
+        const uint32_t from = look.window && t_last >= look.window ? t_last - look.window + 1 : 0;
+        const bool some = tile_tok >= lost && t_first >= from + (BP - 1);
+        const uint32_t full0 = some ? from : 1u << 31, full_reach = some ? t_first - (BP - 1) - from : 0;
         float mx = held ? -CUDART_INF_F : 0.f, unit = 0x1p-100f;          // (a row that sees nothing needs no maximum)
         f2 sum = 0;
         bool ok = true;
+        const uint32_t n = tile < tiles ? nb : 0;
         const f2 sc2 = f2_both(scale);
         auto scale_output = [&](uint32_t j, float corr) {                 // what blocks before j gave
             ok = ok && __all_sync(0xffffffffu, wait(&o_done[tile], (j - 1) & 1, status));
@@ -465,9 +458,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
             for (uint32_t col = 0; col < DIM; col += 32) tmem_st32(at_o + col, zero);
         }
 #pragma unroll 1
-        for (uint32_t j = 0; j < nb; ++j) {
+        for (uint32_t j = 0; j < n; ++j) {
             const uint32_t slot = j % SLOTS, st = j % STAGES, p0 = blocks.at(lo + j) << BP_LOG, at_s = at + (2 * tile + (j & 1)) * BP;
-            const bool full = all_see(look, t_first, t_last, p0, BP) && tile_tok >= lost;
+            const bool full = p0 - full0 <= full_reach;
             ok = wait(&s_full[2 * tile + (j & 1)], (j >> 1) & 1, status);
             if constexpr (CODES) { if (ok) ok = wait(&sc_full[slot], (j / SLOTS) & 1, status); }
             bool odd = false;
@@ -626,9 +619,10 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[2 * tile + (j & 1)]);
+            if (threadIdx.x == 0 && j == 0) mbar_arrive(&apart);
         }
-        if (ok) ok = wait(&o_all[tile], 0, status);
-        ok = __all_sync(0xffffffffu, ok);
+        if (ok && n) ok = wait(&o_all[tile], 0, status);
+        ok = __all_sync(0xffffffffu, ok && n);
         if (ok) {
             tc_fence_after();
             const float l = f2_sum(sum), back = CODES ? unit * (1.0f / UNITS) : 1.0f, inv = sh.chunks > 1 ? back : l == 0.f ? 0.f : back / l;
