@@ -3,16 +3,18 @@
 // Bound by memory: keys and values of a position are read once for all query heads of their KV head and for a tile of up to 16 rows
 // (rows of a sequence times heads of the group), and there are 4 flops a byte and row.  A CTA takes a tile, a KV head and a part of the
 // positions, and each of its warps 16 positions at a time, straight from global memory to registers: pages of 16 and more mean that
-// one page number serves the step.  Scores and weighted values run on m16n8k16 with M = the rows of the tile:
+// one page number serves the step.  Scores and weighted values run on m16n8k16 with N = 8 rows of the tile, transposed:
 //
-//   scores   the order of the contraction over a head's elements is free, so that a lane takes whole 16-byte units of a key
-//            and reads the query's elements in the order that this gives;
-//   values   the weights go from accumulators to the A operand as they lie; B takes the same element of two neighbouring
-//            positions, picked from two 16-byte units with byte permutations.
+//   scores   S^T = K Q^T, M = 16 positions.  The order of the contraction over a head's elements is free, so that a lane takes whole
+//            16-byte units of a key and reads the query's elements in the order that this gives;
+//   values   O^T = V^T P^T, M = 16 elements of the head: the same element of two neighbouring positions, picked from two 16-byte units with
+//            byte permutations.  P^T is S^T's accumulator, rounded to 16 bits and transposed by movmatrix.
 //
-// Codes enter as f16 whole numbers.  Their weights are p * v_scale * 2^12 / U with U a power of two above all value scales of the warp's
-// steps so far, which keeps them inside the f16 range whatever the scales are.  Loads of the next step are under way while this
-// step's products run: the next keys once the scores are done, the next values once the values are.
+// (With the rows as M half of every product is empty for 8 rows and fewer, and each accumulator pair is moved into a group of four.)
+// Codes of keys enter as f16 subnormals, (code + 128) 2^-24, and 128 times the sum of q is taken off again; codes of values as f16 whole
+// numbers.  Their weights are p * v_scale * 256 / U with U a power of two above all value scales of the warp's steps so far, which
+// keeps them inside the f16 range whatever the scales are.  Loads of the next step are under way while this step's products run: the
+// next keys once the scores are done, the next values once the values are.
 #include <math_constants.h>
 
 #include <type_traits>
@@ -25,6 +27,7 @@ using namespace paged;
 namespace {
 
 constexpr uint32_t WARPS = 8, STEP_LOG = 4, STEP = 16;
+constexpr float ROOM = 7.0f, UNITS = 256.0f;       // weights in f16 stay below 2^7 * 256 = 2^15
 
 __device__ __forceinline__ uint4 load16(const void* p) { return __ldcg(static_cast<const uint4*>(p)); }
 
@@ -43,6 +46,14 @@ template <bool CODES> __device__ __forceinline__ uint32_t pack2(float a, float b
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ bool holds_nonfinite(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
+
+// rows and columns of an 8 x 8 matrix of 16-bit numbers exchanged: lane 4 r + t holds columns 2 t, 2 t + 1 of row r
+__device__ __forceinline__ uint32_t transposed(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+__device__ __forceinline__ float2 half_pair(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 
 // a power of two above |v| (v finite), within what 2^12 / U can be
 __device__ __forceinline__ float unit_above(float v) {
@@ -87,28 +98,37 @@ attend_step_kernel(Pool c, Batch b, Look look, uint32_t heads, uint32_t group, c
             *reinterpret_cast<float2*>(part_ml + 2 * (((static_cast<size_t>(span.row0) + u / group) * heads + kvh * group + u % group) * chunks + chunk)) = make_float2(-CUDART_INF_F, 0.f);
         return;
     }
-    // rows of this lane: gid and gid + 8
-    uint32_t at[2];
-    bool held[2];
+    // rows of this lane in scores and output: 2 t, 2 t + 1 (and 8 more)
+    constexpr int NT = TALL ? 2 : 1, LR = 2 * NT;
+    uint32_t at[LR];
+    bool held[LR];
 #pragma unroll
-    for (int i = 0; i < (TALL ? 2 : 1); ++i) {
-        const uint32_t tok = min(u0 + gid + 8 * i, units - 1) / group;
+    for (int i = 0; i < LR; ++i) {
+        const uint32_t tok = min(u0 + 2 * t + (i & 1) + 8 * (i >> 1), units - 1) / group;
         held[i] = tok >= lost;
         at[i] = before + max(tok, lost);
     }
-    float mx[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
-    float o[DIM / 8][TALL ? 4 : 2];
+    float mx[LR], l[LR];
+    float o[NT][DIM / 16][4];                                             // elements e(gid, 2 m), e(gid, 2 m + 1) of rows 2 t, 2 t + 1: [0], [1]; [2], [3]
 #pragma unroll
-    for (int n = 0; n < DIM / 8; ++n)
+    for (int i = 0; i < LR; ++i) { mx[i] = -CUDART_INF_F; l[i] = 0.f; }
 #pragma unroll
-        for (int i = 0; i < (TALL ? 4 : 2); ++i) o[n][i] = 0.f;
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int m = 0; m < DIM / 16; ++m)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[i][m][x] = 0.f;
     bool bad = false, clipped = false;
-    float unit = 0x1p-100f;
+    float unit = 0x1p-100f, per_unit = 0.f;                               // U, UNITS / U
+    // steps that start at full0 .. full0 + full_reach are seen whole by every row (those of the first positions beside a window are not counted here)
+    const uint32_t from = look.window && last >= look.window ? last - look.window + 1 : 0;
+    const bool some = tok0 >= lost && first >= from + (STEP - 1);
+    const uint32_t full0 = some ? from : 1u << 31, full_reach = some ? first - (STEP - 1) - from : 0;
 
     if (lo + warp < hi) {
-        uint32_t qa[KS][TALL ? 4 : 2];
+        uint32_t qa[NT][KS][2];
 #pragma unroll
-        for (int i = 0; i < (TALL ? 2 : 1); ++i) {
+        for (int i = 0; i < NT; ++i) {
             const uint32_t u = u0 + gid + 8 * i;
             const Q* row = q + static_cast<size_t>(span.row0 + (u < units ? u / group : 0)) * ldq + (static_cast<size_t>(kvh) * group + (u < units ? u % group : 0)) * DIM;
 #pragma unroll
@@ -128,145 +148,160 @@ attend_step_kernel(Pool c, Batch b, Look look, uint32_t heads, uint32_t group, c
                     if constexpr (CODES)
                         for (int x = 0; x < 4; ++x) { clipped |= fabsf(e[x]) > 65504.0f; e[x] = fabsf(e[x]) > 65504.0f ? copysignf(65504.0f, e[x]) : e[x]; }
                 }
-                qa[j][i] = pack2<CODES>(e[0], e[1]);
-                qa[j][(TALL ? 2 : 1) + i] = pack2<CODES>(e[2], e[3]);
+                qa[i][j][0] = pack2<CODES>(e[0], e[1]);
+                qa[i][j][1] = pack2<CODES>(e[2], e[3]);
+            }
+        }
+        float q128[LR];                                                   // 128 times what a row of q adds up to: codes enter as code + 128
+        if constexpr (CODES) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                float sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < KS; ++j) {
+                    const float2 x = half_pair(qa[i][j][0]), y = half_pair(qa[i][j][1]);
+                    sum += (x.x + x.y) + (y.x + y.y);
+                }
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+                for (int x = 0; x < 2; ++x) q128[2 * i + x] = 128.0f * __shfl_sync(0xffffffffu, sum, 4 * (2 * t + x));
             }
         }
         uint4 kr[2][KU];
         uint32_t vr[4][VU][VW];
-        float ks[4], vs[4];
-        auto base_of = [&](uint32_t step) {                               // first row of the step's positions in this head
+        float ks[2], vs[2];                                               // of positions gid, gid + 8
+        const uint8_t *k_at = static_cast<const uint8_t*>(c.k) + gid * ROW + 16 * t, *v_at = static_cast<const uint8_t*>(c.v) + 2 * t * ROW + gid * (VW * 4);
+        const float *ks_at = CODES ? c.k_scale + gid : nullptr, *vs_at = CODES ? c.v_scale + gid : nullptr;
+        auto place = [&](uint32_t step) {                                 // where the step's positions lie in this head, in sixteens of rows
             const uint32_t p = blocks.at(step) << STEP_LOG;
-            return c.row(page_of(c, b, s, p, bad), kvh, p & (c.size() - 1));
+            return ((page_of(c, b, s, p, bad) * c.kv_heads + kvh) << (c.shift - STEP_LOG)) + ((p & (c.size() - 1)) >> STEP_LOG);
         };
-        auto load_k = [&](size_t base) {
+        auto load_k = [&](uint32_t at16) {
+            const uint8_t* rows = k_at + static_cast<uint64_t>(at16) * (STEP * ROW);
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
-                for (int i = 0; i < KU; ++i) kr[n][i] = load16(static_cast<const uint8_t*>(c.k) + (base + 8 * n + gid) * ROW + (4 * i + t) * 16);
+                for (int i = 0; i < KU; ++i) kr[n][i] = load16(rows + 8 * n * ROW + 64 * i);
             if constexpr (CODES) {
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const float2 a = __ldcg(reinterpret_cast<const float2*>(c.k_scale + base + 8 * n) + t);
-                    ks[2 * n] = a.x; ks[2 * n + 1] = a.y;
-                }
+                const float* sc = ks_at + static_cast<uint64_t>(at16) * STEP;
+                ks[0] = __ldcg(sc);
+                ks[1] = __ldcg(sc + 8);
             }
         };
-        auto load_v = [&](size_t base) {
+        auto load_v = [&](uint32_t at16) {
+            const uint8_t* from = v_at + static_cast<uint64_t>(at16) * (STEP * ROW);
 #pragma unroll
             for (int x = 0; x < 4; ++x)
 #pragma unroll
                 for (int i = 0; i < VU; ++i) {
-                    const uint8_t* from = static_cast<const uint8_t*>(c.v) + (base + 2 * t + (x & 1) + 8 * (x >> 1)) * ROW + (gid + 8 * i) * (VW * 4);
-                    if constexpr (VW == 4) { const uint4 w = load16(from); vr[x][i][0] = w.x; vr[x][i][1] = w.y; vr[x][i][2] = w.z; vr[x][i][3] = w.w; }
-                    else { const uint2 w = __ldcg(reinterpret_cast<const uint2*>(from)); vr[x][i][0] = w.x; vr[x][i][1] = w.y; }
+                    const uint8_t* here = from + ((x & 1) + 8 * (x >> 1)) * ROW + 8 * i * (VW * 4);
+                    if constexpr (VW == 4) { const uint4 w = load16(here); vr[x][i][0] = w.x; vr[x][i][1] = w.y; vr[x][i][2] = w.z; vr[x][i][3] = w.w; }
+                    else { const uint2 w = __ldcg(reinterpret_cast<const uint2*>(here)); vr[x][i][0] = w.x; vr[x][i][1] = w.y; }
                 }
             if constexpr (CODES) {
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const float2 a = __ldcg(reinterpret_cast<const float2*>(c.v_scale + base + 8 * n) + t);
-                    vs[2 * n] = a.x; vs[2 * n + 1] = a.y;
-                }
+                const float* sc = vs_at + static_cast<uint64_t>(at16) * STEP;
+                vs[0] = __ldcg(sc);
+                vs[1] = __ldcg(sc + 8);
             }
         };
-        uint32_t step = lo + warp;
-        size_t base = base_of(step), next = step + WARPS < hi ? base_of(step + WARPS) : base;
-        load_k(base);
-        load_v(base);
+        uint32_t step = lo + warp, here = place(step), next = step + WARPS < hi ? place(step + WARPS) : here;
+        load_k(here);
+        load_v(here);
+#pragma unroll 1
         for (; step < hi; step += WARPS) {
             const uint32_t p0 = blocks.at(step) << STEP_LOG;
-            const bool more = step + WARPS < hi;
-            // ---- scores: n-tile n holds positions p0 + 8 n + 2 t, + 1 of rows gid (and gid + 8)
-            float sc[2][4];
+            const bool more = step + WARPS < hi, full = p0 - full0 <= full_reach;
+            const uint32_t later = step + 2 * WARPS < hi ? place(step + 2 * WARPS) : next;
+            // ---- scores: sc[i][2 n + x] of position p0 + gid + 8 n and row 2 t + x + 8 i
+            float sc[NT][4];
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                float a[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < NT; ++i) sc[i][0] = sc[i][1] = sc[i][2] = sc[i][3] = 0.f;
 #pragma unroll
-                for (int i = 0; i < KU; ++i) {
-                    const uint32_t w[4] = {kr[n][i].x, kr[n][i].y, kr[n][i].z, kr[n][i].w};
-                    if constexpr (CODES) {
-                        const __half2 bias = __float2half2_rn(1152.0f);
+            for (int i = 0; i < KU; ++i) {
+                const uint32_t a[4] = {kr[0][i].x, kr[0][i].y, kr[0][i].z, kr[0][i].w}, e[4] = {kr[1][i].x, kr[1][i].y, kr[1][i].z, kr[1][i].w};
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const uint32_t y = w[x] ^ 0x80808080u;
-                            const uint32_t(&f)[TALL ? 4 : 2] = qa[4 * i + x];
-                            mma<true>(a, f[0], TALL ? f[1] : 0u, f[TALL ? 2 : 1], TALL ? f[TALL ? 3 : 0] : 0u, tc::h2_bits(tc::codes01(y, bias)), tc::h2_bits(tc::codes23(y, bias)));
-                        }
+                for (int x = 0; x < (CODES ? 4 : 2); ++x) {
+                    uint32_t f[4];
+                    if constexpr (CODES) {                                // code + 128 in every byte: with a byte of zeros above an f16 of 2^-24 times that
+                        const uint32_t y = a[x] ^ 0x80808080u, z = e[x] ^ 0x80808080u;
+                        f[0] = __byte_perm(y, 0u, 0x4140u); f[1] = __byte_perm(z, 0u, 0x4140u);
+                        f[2] = __byte_perm(y, 0u, 0x4342u); f[3] = __byte_perm(z, 0u, 0x4342u);
                     } else {
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const uint32_t(&f)[TALL ? 4 : 2] = qa[2 * i + x];
-                            mma<false>(a, f[0], TALL ? f[1] : 0u, f[TALL ? 2 : 1], TALL ? f[TALL ? 3 : 0] : 0u, w[2 * x], w[2 * x + 1]);
-                        }
+                        f[0] = a[(2 * x) & 3]; f[1] = e[(2 * x) & 3]; f[2] = a[(2 * x + 1) & 3]; f[3] = e[(2 * x + 1) & 3];
                     }
+#pragma unroll
+                    for (int r = 0; r < NT; ++r) mma<CODES>(sc[r], f[0], f[1], f[2], f[3], qa[r][(CODES ? 4 : 2) * i + x][0], qa[r][(CODES ? 4 : 2) * i + x][1]);
                 }
-                float f0 = look.scale, f1 = look.scale;
-                if constexpr (CODES) { f0 *= ks[2 * n]; f1 *= ks[2 * n + 1]; }
-                sc[n][0] = a[0] * f0; sc[n][1] = a[1] * f1; sc[n][2] = a[2] * f0; sc[n][3] = a[3] * f1;
             }
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    if constexpr (CODES) sc[i][x] = fmaf(sc[i][x], 0x1p24f, -q128[2 * i + (x & 1)]) * (look.scale * ks[x >> 1]);
+                    else sc[i][x] *= look.scale;
+                }
             if (more) load_k(next);
             // ---- what the rows do not see
-            const bool full = all_see(look, first, last, p0, STEP) && tok0 >= lost;
-            uint32_t seen = 0xffu;                                        // bit 4 i + 2 n + x: row i, position p0 + 8 n + 2 t + x
+            uint32_t seen = 0xffu;                                        // bit 4 i + x, as in sc
             if (!full) {
                 seen = 0;
 #pragma unroll
-                for (int i = 0; i < (TALL ? 2 : 1); ++i)
+                for (int i = 0; i < NT; ++i)
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const bool yes = held[i] && look.sees(at[i], p0 + 8 * n + 2 * t + x);
-                            seen |= static_cast<uint32_t>(yes) << (4 * i + 2 * n + x);
-                            if (!yes) sc[n][2 * i + x] = -CUDART_INF_F;
-                        }
-            }
-            // ---- softmax: maximum and sum so far of each row
-            float w[2][4], corr[2] = {1.f, 1.f};
-#pragma unroll
-            for (int i = 0; i < (TALL ? 2 : 1); ++i) {
-                float top = fmaxf(fmaxf(sc[0][2 * i], sc[0][2 * i + 1]), fmaxf(sc[1][2 * i], sc[1][2 * i + 1]));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float to = fmaxf(mx[i], top), zero = to == -CUDART_INF_F ? 0.f : to;
-                corr[i] = tc::ex2(mx[i] - zero);
-                mx[i] = to;
-                float sum = 0.f;
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        w[n][2 * i + x] = tc::ex2(sc[n][2 * i + x] - zero);
-                        sum += w[n][2 * i + x];
+                    for (int x = 0; x < 4; ++x) {
+                        const bool yes = held[2 * i + (x & 1)] && look.sees(at[2 * i + (x & 1)], p0 + gid + 8 * (x >> 1));
+                        seen |= static_cast<uint32_t>(yes) << (4 * i + x);
+                        if (!yes) sc[i][x] = -CUDART_INF_F;
                     }
-                l[i] = l[i] * corr[i] + sum;                              // (of this lane's positions; the lanes of a row are added at the end)
             }
-            if constexpr (CODES) {
-                float top = 0.f;
+            // ---- softmax against the maximum of earlier steps, as long as no score passes it by more than 2^ROOM, and no value scale passes U
+            bool change = false;
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+            for (int i = 0; i < LR; ++i) change |= fmaxf(sc[i >> 1][i & 1], sc[i >> 1][2 + (i & 1)]) > mx[i] + ROOM;
+            if constexpr (CODES) change |= fmaxf(fabsf(vs[0]), fabsf(vs[1])) >= unit;
+            if (__any_sync(0xffffffffu, change)) {
+                float corr[LR];
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const float a = fabsf(vs[2 * n + x]);
-                        if (a < CUDART_INF_F && (full || some_see(look, first, last, p0 + 8 * n + 2 * t + x))) top = fmaxf(top, a);
-                    }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float above = fmaxf(unit, unit_above(top)), f = 4096.0f / above;
-                if (above != unit) { corr[0] *= unit / above; corr[1] *= unit / above; unit = above; }
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int x = 0; x < (TALL ? 4 : 2); ++x) w[n][x] = (seen >> (4 * (x >> 1) + 2 * n + (x & 1))) & 1 ? w[n][x] * (vs[2 * n + (x & 1)] * f) : 0.f;
-            }
-            const bool rescale = corr[0] != 1.f || (TALL && corr[1] != 1.f);
-            if (__any_sync(0xffffffffu, rescale)) {
-#pragma unroll
-                for (int n = 0; n < DIM / 8; ++n) {
-                    o[n][0] *= corr[0]; o[n][1] *= corr[0];
-                    if constexpr (TALL) { o[n][2] *= corr[1]; o[n][3] *= corr[1]; }
+                for (int i = 0; i < LR; ++i) {
+                    float top = fmaxf(sc[i >> 1][i & 1], sc[i >> 1][2 + (i & 1)]);
+                    for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    const float to = fmaxf(mx[i], top);
+                    corr[i] = tc::ex2(mx[i] - (to == -CUDART_INF_F ? 0.f : to));
+                    mx[i] = to;
+                    l[i] *= corr[i];
                 }
+                if constexpr (CODES) {
+                    float large = 0.f;
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        const float a = fabsf(vs[n]);
+                        if (a < CUDART_INF_F && (full || some_see(look, first, last, p0 + gid + 8 * n))) large = fmaxf(large, a);
+                    }
+                    for (int d = 4; d < 32; d <<= 1) large = fmaxf(large, __shfl_xor_sync(0xffffffffu, large, d));
+                    const float above = fmaxf(unit, unit_above(large));
+#pragma unroll
+                    for (int i = 0; i < LR; ++i) corr[i] *= unit / above;
+                    unit = above;
+                    per_unit = UNITS / above;
+                }
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int m = 0; m < DIM / 16; ++m)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) o[i][m][x] *= corr[2 * i + (x & 1)];
             }
+            float w[NT][4];
+            const float v0 = vs[0] * per_unit, v1 = vs[1] * per_unit;
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const float top = mx[2 * i + (x & 1)], e = tc::ex2(sc[i][x] - (top == -CUDART_INF_F ? 0.f : top));
+                    l[2 * i + (x & 1)] += e;                              // (of this lane's positions; the lanes of a row are added at the end)
+                    w[i][x] = CODES ? ((seen >> (4 * i + x)) & 1 ? e * (x >> 1 ? v1 : v0) : 0.f) : e;
+                }
             // ---- values
             bool odd = false;                                             // infinities or NaN among values that some of the rows do not see
             if constexpr (!CODES) {
@@ -286,13 +321,15 @@ attend_step_kernel(Pool c, Batch b, Look look, uint32_t heads, uint32_t group, c
                 }
             }
             if (!odd) {
-                const uint32_t a0 = pack2<CODES>(w[0][0], w[0][1]), a2 = pack2<CODES>(w[1][0], w[1][1]);
-                const uint32_t a1 = TALL ? pack2<CODES>(w[0][2], w[0][3]) : 0u, a3 = TALL ? pack2<CODES>(w[1][2], w[1][3]) : 0u;
-                auto add = [&](int n, uint32_t b0, uint32_t b1) {
-                    float d[4] = {o[n][0], o[n][1], TALL ? o[n][TALL ? 2 : 0] : 0.f, TALL ? o[n][TALL ? 3 : 0] : 0.f};
-                    mma<CODES>(d, a0, a1, a2, a3, b0, b1);
+                uint32_t b0[NT], b1[NT];
 #pragma unroll
-                    for (int x = 0; x < (TALL ? 4 : 2); ++x) o[n][x] = d[x];
+                for (int i = 0; i < NT; ++i) {
+                    b0[i] = transposed(pack2<CODES>(w[i][0], w[i][1]));
+                    b1[i] = transposed(pack2<CODES>(w[i][2], w[i][3]));
+                }
+                auto add = [&](int m, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) mma<CODES>(o[i][m], a0, a1, a2, a3, b0[i], b1[i]);
                 };
 #pragma unroll
                 for (int i = 0; i < VU; ++i)
@@ -304,58 +341,53 @@ attend_step_kernel(Pool c, Batch b, Look look, uint32_t heads, uint32_t group, c
                             const __half2 bias = __float2half2_rn(1152.0f);
                             const uint32_t lo01 = __byte_perm(va, vb, 0x5140u) ^ 0x80808080u, hi01 = __byte_perm(va, vb, 0x7362u) ^ 0x80808080u;
                             const uint32_t lo89 = __byte_perm(vc, vd, 0x5140u) ^ 0x80808080u, hi89 = __byte_perm(vc, vd, 0x7362u) ^ 0x80808080u;
-                            const int n = i * VE + 4 * y;
-                            add(n, tc::h2_bits(tc::codes01(lo01, bias)), tc::h2_bits(tc::codes01(lo89, bias)));
-                            add(n + 1, tc::h2_bits(tc::codes23(lo01, bias)), tc::h2_bits(tc::codes23(lo89, bias)));
-                            add(n + 2, tc::h2_bits(tc::codes01(hi01, bias)), tc::h2_bits(tc::codes01(hi89, bias)));
-                            add(n + 3, tc::h2_bits(tc::codes23(hi01, bias)), tc::h2_bits(tc::codes23(hi89, bias)));
+                            const int m = (i * VE + 4 * y) / 2;
+                            add(m, tc::h2_bits(tc::codes01(lo01, bias)), tc::h2_bits(tc::codes23(lo01, bias)), tc::h2_bits(tc::codes01(lo89, bias)), tc::h2_bits(tc::codes23(lo89, bias)));
+                            add(m + 1, tc::h2_bits(tc::codes01(hi01, bias)), tc::h2_bits(tc::codes23(hi01, bias)), tc::h2_bits(tc::codes01(hi89, bias)), tc::h2_bits(tc::codes23(hi89, bias)));
                         } else {
-                            const int n = i * VE + 2 * y;
-                            add(n, __byte_perm(va, vb, 0x5410u), __byte_perm(vc, vd, 0x5410u));
-                            add(n + 1, __byte_perm(va, vb, 0x7632u), __byte_perm(vc, vd, 0x7632u));
+                            add((i * VE + 2 * y) / 2, __byte_perm(va, vb, 0x5410u), __byte_perm(va, vb, 0x7632u), __byte_perm(vc, vd, 0x5410u), __byte_perm(vc, vd, 0x7632u));
                         }
                     }
             } else if constexpr (!CODES) {
                 // 0 times infinity is not 0: each row adds up the positions that it sees, one by one
-                const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(c.v) + base * DIM;
+                const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(c.v) + static_cast<uint64_t>(here) * (STEP * DIM);
 #pragma unroll 1
                 for (uint32_t p = 0; p < STEP; ++p) {
-                    const uint32_t from = (lane & ~3u) | ((p & 7) >> 1);
 #pragma unroll
-                    for (int i = 0; i < (TALL ? 2 : 1); ++i) {
-                        const float a = p & 1 ? (p < 8 ? w[0][2 * i + 1] : w[1][2 * i + 1]) : (p < 8 ? w[0][2 * i] : w[1][2 * i]);
-                        const float weight = __shfl_sync(0xffffffffu, a, from);
+                    for (int i = 0; i < LR; ++i) {
+                        const float weight = __shfl_sync(0xffffffffu, p < 8 ? w[i >> 1][i & 1] : w[i >> 1][2 + (i & 1)], 4 * (p & 7) + t);
                         if (held[i] && look.sees(at[i], p0 + p)) {
 #pragma unroll
-                            for (int n = 0; n < DIM / 8; ++n)
-#pragma unroll
-                                for (int x = 0; x < 2; ++x)
-                                    o[n][2 * i + x] = fmaf(weight, __bfloat162float(v[p * DIM + (2 * t + x + 8 * (n / VE)) * VE + n % VE]), o[n][2 * i + x]);
+                            for (int e = 0; e < DIM / 8; ++e) {
+                                float& to = o[i >> 1][e / 2][2 * (e & 1) + (i & 1)];
+                                to = fmaf(weight, __bfloat162float(v[p * DIM + (gid + 8 * (e / VE)) * VE + e % VE]), to);
+                            }
                         }
                     }
                 }
+                __syncwarp();
             }
             if (more) {
                 load_v(next);
-                base = next;
-                if (step + 2 * WARPS < hi) next = base_of(step + 2 * WARPS);
+                here = next;
+                next = later;
             }
         }
     }
     // ---- the warps' rows meet in shared memory
-    const float back = CODES ? unit * (1.0f / 4096.0f) : 1.0f;
+    const float back = CODES ? unit * (1.0f / UNITS) : 1.0f;
 #pragma unroll
-    for (int i = 0; i < (TALL ? 2 : 1); ++i) {
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        if (t == 0) { red_m[warp][gid + 8 * i] = mx[i]; red_l[warp][gid + 8 * i] = l[i]; }
-        float* mine = red + (warp * R + gid + 8 * i) * (DIM + 4);
+    for (int i = 0; i < LR; ++i) {
+        const uint32_t r = 2 * t + (i & 1) + 8 * (i >> 1);
+        for (int d = 4; d < 32; d <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], d);
+        if (gid == 0) { red_m[warp][r] = mx[i]; red_l[warp][r] = l[i]; }
+        float* row = red + (warp * R + r) * (DIM + 4);
 #pragma unroll
-        for (int n = 0; n < DIM / 8; n += 4)
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-                *reinterpret_cast<float4*>(mine + (2 * t + x + 8 * (n / VE)) * VE + n % VE) =
-                    make_float4(o[n][2 * i + x] * back, o[n + 1][2 * i + x] * back, o[n + 2][2 * i + x] * back, o[n + 3][2 * i + x] * back);
+        for (int e = 0; e < DIM / 8; e += 4) {
+            const float (*x)[4] = o[i >> 1] + e / 2;
+            *reinterpret_cast<float4*>(row + (gid + 8 * (e / VE)) * VE + e % VE) =
+                make_float4(x[0][i & 1] * back, x[0][2 + (i & 1)] * back, x[1][i & 1] * back, x[1][2 + (i & 1)] * back);
+        }
     }
     __syncthreads();
     constexpr int LANES = DIM / 4;                                        // threads of a row, four elements each
