@@ -8,6 +8,7 @@
 #include <math_constants.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "paged_common.cuh"
 
@@ -69,16 +70,29 @@ Plan plan_of(const hf2q_pages& c, const hf2q_page_batch& b, uint32_t heads, uint
     const uint64_t group = heads / c.kv_heads, units = b.max_new * group;
     p.step = units <= STEP_UNITS;
     const uint64_t rows = units <= 8 ? 8 : p.step ? 16 : 2 * (128 / group) * group;
-    // most positions that a tile goes through; and tiles, as if every sequence that can have rows had the most
-    uint64_t seen = (b.max_length + 127ull) / 128 * 128;
-    if (window) seen = std::min<uint64_t>(seen, (static_cast<uint64_t>(window) + b.max_new + sinks + 256 + 127) / 128 * 128);
-    const uint64_t tiles = static_cast<uint64_t>(c.kv_heads) * std::min(b.seqs, b.rows) * ((units + rows - 1) / rows);
-    // One part for each place that a CTA can have; several sequences are of several lengths, and smaller parts even them out.
-    const uint64_t places = (p.step ? 2ull : 1ull) * sms * (b.seqs > 1 && p.step ? 4 : 1);
-    uint64_t chunk = std::max<uint64_t>(p.step ? 256 : 512, (tiles * seen + places - 1) / places);
-    if (!p.step && tiles >= places) chunk = seen;
-    chunk = std::max(chunk, (seen + 255) / 256);
-    chunk = (chunk + 127) / 128 * 128;
+    // most positions that a tile goes through, and tiles as if every sequence that can have rows had the most
+    const uint64_t ceil128 = (b.max_length + 127ull) / 128 * 128, seqs = std::min(b.seqs, b.rows);
+    uint64_t seen = ceil128;
+    if (window) seen = std::min<uint64_t>(seen, (static_cast<uint64_t>(window) + b.max_new + sinks + (p.step ? 32 : 256) + 127) / 128 * 128);
+    const uint64_t tiles = static_cast<uint64_t>(c.kv_heads) * seqs * ((units + rows - 1) / rows);
+    uint64_t chunk = seen;
+    if (p.step) {
+        // A CTA takes about 4 us to begin and end and 1 us for 64 positions, two CTAs run on an SM, and joining parts takes 3 us.  One sequence: whole
+        // rounds of equal parts.  Several, of several lengths: what they hold together, six tenths of the most (all of it in a window), shared evenly,
+        // and half of one part for the end.  (Of 24 sequences with a window of 1024 in 64 elements: parts of 256 positions 26 us, whole 15 us.)
+        const double places = 2.0 * sms, held = seqs == 1 || seen < ceil128 ? 1.0 : 0.6;
+        double best = 0.0;
+        for (uint64_t parts = 1; parts <= 256 && (parts == 1 || seen / parts >= 128); ++parts) {
+            const uint64_t size = ((seen + parts - 1) / parts + 127) / 128 * 128;
+            const double one = 4.0 + size / 64.0, all = tiles * held * (4.0 * parts + seen / 64.0), join = parts > 1 ? 3.0 : 0.0;
+            const double cost = (seqs == 1 ? std::ceil(tiles * parts / places) * one : std::max(one, all / places + 0.5 * one)) + join;
+            if (parts == 1 || cost < best) { best = cost; chunk = size; }
+        }
+    } else if (tiles < static_cast<uint64_t>(sms)) {
+        // few tiles: a part for each SM, of no fewer than eight blocks
+        chunk = std::max<uint64_t>(512, (tiles * seen + sms - 1) / sms);
+        chunk = (std::max(chunk, (seen + 255) / 256) + 127) / 128 * 128;
+    }
     p.chunks = static_cast<uint32_t>((seen + chunk - 1) / chunk);
     p.chunk = static_cast<uint32_t>(chunk);
     p.scratch = p.chunks > 1 ? (static_cast<uint64_t>(b.rows) * heads * p.chunks * (c.dim + 2) * 4 + 255) / 256 * 256 : 256;

@@ -126,6 +126,47 @@ attend_step_kernel(Pool c, Batch b, Look look, uint32_t heads, uint32_t group, c
     const uint32_t full0 = some ? from : 1u << 31, full_reach = some ? first - (STEP - 1) - from : 0;
 
     if (lo + warp < hi) {
+        // keys and values first: their page and they themselves are two trips to memory, q one
+        uint4 kr[2][KU];
+        uint32_t vr[4][VU][VW];
+        float ks[2], vs[2];                                               // of positions gid, gid + 8
+        const uint8_t *k_at = static_cast<const uint8_t*>(c.k) + gid * ROW + 16 * t, *v_at = static_cast<const uint8_t*>(c.v) + 2 * t * ROW + gid * (VW * 4);
+        const float *ks_at = CODES ? c.k_scale + gid : nullptr, *vs_at = CODES ? c.v_scale + gid : nullptr;
+        auto place = [&](uint32_t step) {                                 // where the step's positions lie in this head, in sixteens of rows
+            const uint32_t p = blocks.at(step) << STEP_LOG;
+            return ((page_of(c, b, s, p, bad) * c.kv_heads + kvh) << (c.shift - STEP_LOG)) + ((p & (c.size() - 1)) >> STEP_LOG);
+        };
+        auto load_k = [&](uint32_t at16) {
+            const uint8_t* rows = k_at + static_cast<uint64_t>(at16) * (STEP * ROW);
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < KU; ++i) kr[n][i] = load16(rows + 8 * n * ROW + 64 * i);
+            if constexpr (CODES) {
+                const float* sc = ks_at + static_cast<uint64_t>(at16) * STEP;
+                ks[0] = __ldcg(sc);
+                ks[1] = __ldcg(sc + 8);
+            }
+        };
+        auto load_v = [&](uint32_t at16) {
+            const uint8_t* from = v_at + static_cast<uint64_t>(at16) * (STEP * ROW);
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int i = 0; i < VU; ++i) {
+                    const uint8_t* here = from + ((x & 1) + 8 * (x >> 1)) * ROW + 8 * i * (VW * 4);
+                    if constexpr (VW == 4) { const uint4 w = load16(here); vr[x][i][0] = w.x; vr[x][i][1] = w.y; vr[x][i][2] = w.z; vr[x][i][3] = w.w; }
+                    else { const uint2 w = __ldcg(reinterpret_cast<const uint2*>(here)); vr[x][i][0] = w.x; vr[x][i][1] = w.y; }
+                }
+            if constexpr (CODES) {
+                const float* sc = vs_at + static_cast<uint64_t>(at16) * STEP;
+                vs[0] = __ldcg(sc);
+                vs[1] = __ldcg(sc + 8);
+            }
+        };
+        uint32_t step = lo + warp, here = place(step), next = step + WARPS < hi ? place(step + WARPS) : here;
+        load_k(here);
+        load_v(here);
         uint32_t qa[NT][KS][2];
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
@@ -168,46 +209,6 @@ attend_step_kernel(Pool c, Batch b, Look look, uint32_t heads, uint32_t group, c
                 for (int x = 0; x < 2; ++x) q128[2 * i + x] = 128.0f * __shfl_sync(0xffffffffu, sum, 4 * (2 * t + x));
             }
         }
-        uint4 kr[2][KU];
-        uint32_t vr[4][VU][VW];
-        float ks[2], vs[2];                                               // of positions gid, gid + 8
-        const uint8_t *k_at = static_cast<const uint8_t*>(c.k) + gid * ROW + 16 * t, *v_at = static_cast<const uint8_t*>(c.v) + 2 * t * ROW + gid * (VW * 4);
-        const float *ks_at = CODES ? c.k_scale + gid : nullptr, *vs_at = CODES ? c.v_scale + gid : nullptr;
-        auto place = [&](uint32_t step) {                                 // where the step's positions lie in this head, in sixteens of rows
-            const uint32_t p = blocks.at(step) << STEP_LOG;
-            return ((page_of(c, b, s, p, bad) * c.kv_heads + kvh) << (c.shift - STEP_LOG)) + ((p & (c.size() - 1)) >> STEP_LOG);
-        };
-        auto load_k = [&](uint32_t at16) {
-            const uint8_t* rows = k_at + static_cast<uint64_t>(at16) * (STEP * ROW);
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int i = 0; i < KU; ++i) kr[n][i] = load16(rows + 8 * n * ROW + 64 * i);
-            if constexpr (CODES) {
-                const float* sc = ks_at + static_cast<uint64_t>(at16) * STEP;
-                ks[0] = __ldcg(sc);
-                ks[1] = __ldcg(sc + 8);
-            }
-        };
-        auto load_v = [&](uint32_t at16) {
-            const uint8_t* from = v_at + static_cast<uint64_t>(at16) * (STEP * ROW);
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-#pragma unroll
-                for (int i = 0; i < VU; ++i) {
-                    const uint8_t* here = from + ((x & 1) + 8 * (x >> 1)) * ROW + 8 * i * (VW * 4);
-                    if constexpr (VW == 4) { const uint4 w = load16(here); vr[x][i][0] = w.x; vr[x][i][1] = w.y; vr[x][i][2] = w.z; vr[x][i][3] = w.w; }
-                    else { const uint2 w = __ldcg(reinterpret_cast<const uint2*>(here)); vr[x][i][0] = w.x; vr[x][i][1] = w.y; }
-                }
-            if constexpr (CODES) {
-                const float* sc = vs_at + static_cast<uint64_t>(at16) * STEP;
-                vs[0] = __ldcg(sc);
-                vs[1] = __ldcg(sc + 8);
-            }
-        };
-        uint32_t step = lo + warp, here = place(step), next = step + WARPS < hi ? place(step + WARPS) : here;
-        load_k(here);
-        load_v(here);
 #pragma unroll 1
         for (; step < hi; step += WARPS) {
             const uint32_t p0 = blocks.at(step) << STEP_LOG;

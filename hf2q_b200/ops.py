@@ -77,6 +77,10 @@ class GgmlQuantizedMatmulIdParams:
     ggml_type: int
 
 
+# torch's current stream as a number, without an object around it where torch says it that way (each call of this package asks)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 class GpuContext:
     """One device context (serve/gpu.rs:19-38).  Not shared between threads."""
 
@@ -107,7 +111,7 @@ class GpuContext:
             raise Hf2qError(rc, self._lib.hf2q_cuda_last_error(self._h).decode())
 
     def _stream(self) -> int:
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return _raw_stream(self.device)
 
     def check_status(self) -> None:
         """Synchronises the current stream and raises if a kernel flagged a problem."""

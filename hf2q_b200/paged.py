@@ -42,14 +42,18 @@ def _on_device(t: torch.Tensor, name: str, dtypes, ctx, contiguous: bool = True)
 
 
 def _rows(t: torch.Tensor, name: str, dtypes, rows: int, width: int, ctx) -> int:
-    """Checks a matrix whose rows may lie further apart than they are wide; returns their distance."""
+    """Checks a matrix whose rows may lie further apart than they are wide; returns their distance.  (On the way of every call: what is
+    right is seen with few questions.)"""
+    if t.dtype in dtypes and t.get_device() == ctx.device and t.dim() == 2:
+        (n, w), (ld, one) = t.shape, t.stride()
+        if n >= rows and w >= width and (one == 1 or w <= 1) and (ld >= width or rows <= 1):
+            return ld if rows > 1 else max(ld, width)
     _on_device(t, name, dtypes, ctx, contiguous=False)
-    if t.dim() != 2 or t.shape[0] < rows or t.shape[1] < width or (t.shape[1] > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < width):
-        _refuse(f"{name} must hold {rows} rows of {width} elements side by side")
-    return t.stride(0) if rows > 1 else max(t.stride(0), width)
+    _refuse(f"{name} must hold {rows} rows of {width} elements side by side")
 
 
 _INT = (torch.int32, torch.uint32)
+_IN, _OUT = (torch.float32, torch.bfloat16), (torch.float32, torch.bfloat16, torch.float16)
 
 
 def rope_frequencies(rot_dim: int, theta: float, *, linear: float = 1.0, bands: dict | None = None) -> torch.Tensor:
@@ -71,7 +75,9 @@ class Rope:
     def __init__(self, freq: torch.Tensor, halves: bool = False, factor: float = 1.0):
         if freq.dtype != torch.float32 or not freq.is_cuda or not freq.is_contiguous() or freq.dim() != 1:
             _refuse("freq must be a contiguous float32 vector on the device")
-        self.freq, self.halves, self.factor = freq, bool(halves), float(factor)
+        self.freq, self.halves, self.factor, self.device = freq, bool(halves), float(factor), freq.get_device()
+        self._plain = self.struct(None)
+        self.ref = C.byref(self._plain)
 
     def struct(self, positions: torch.Tensor | None) -> _Rotary:
         return _Rotary(self.freq.data_ptr(), None if positions is None else positions.data_ptr(), 2 * self.freq.numel(), int(self.halves), self.factor)
@@ -97,14 +103,15 @@ class PagedBatch:
         self.rows, self.max_new, self.max_length = int(rows), int(max_new), int(max_length)
         self.struct = _PageBatch(start.data_ptr(), length.data_ptr(), table.data_ptr(), seqs, self.rows, table.stride(0) if seqs > 1 else table.shape[1],
                                  self.max_new, self.max_length)
-        self._scratch: dict = {}
+        self.ref, self._scratch = C.byref(self.struct), {}
 
     def scratch(self, pages: _Pages, heads: int, window: int, sinks: int) -> torch.Tensor:
+        """Scratch of attention calls of these sizes."""
         key = (pages.kv_heads, pages.dim, pages.dtype, pages.page, heads, window, sinks)
         buf = self._scratch.get(key)
         if buf is None:
             need = C.c_uint64()
-            self.ctx._check(self.ctx._lib.hf2q_cuda_pages_attend_scratch_bytes(self.ctx._h, C.byref(pages), C.byref(self.struct), heads, window, sinks, C.byref(need)))
+            self.ctx._check(self.ctx._lib.hf2q_cuda_pages_attend_scratch_bytes(self.ctx._h, C.byref(pages), self.ref, heads, window, sinks, C.byref(need)))
             buf = self._scratch[key] = torch.empty(max(need.value, 256), dtype=torch.uint8, device=torch.device("cuda", self.ctx.device))
         return buf
 
@@ -130,6 +137,8 @@ class PagedCache:
         at = lambda t, layer: None if t is None else t[layer].data_ptr()
         self._structs = [_Pages(at(k, i), at(v, i), at(k_scale, i), at(v_scale, i), self.pages, self.page, self.kv_heads, self.dim, DT_I8 if codes else DT_BF16)
                          for i in range(self.layers)]
+        self._refs, self._scale = [C.byref(s) for s in self._structs], self.dim ** -0.5
+        self._append, self._attend = ctx._lib.hf2q_cuda_pages_append, ctx._lib.hf2q_cuda_pages_attend
 
     @classmethod
     def allocate(cls, ctx: ops.GpuContext, layers: int, pages: int, page: int, kv_heads: int, dim: int, dtype=torch.int8) -> "PagedCache":
@@ -138,43 +147,42 @@ class PagedCache:
         scales = [torch.zeros((layers, pages, kv_heads, page), dtype=torch.float32, device=dev) for _ in "kv"] if dtype == torch.int8 else [None, None]
         return cls(ctx, *kv, *scales)
 
-    def _layer(self, layer: int) -> _Pages:
+    def _check(self, layer: int, batch: PagedBatch) -> None:
         if not 0 <= layer < self.layers:
             _refuse(f"layer {layer} of {self.layers}")
-        return self._structs[layer]
-
-    def _same(self, batch: PagedBatch) -> None:
         if batch.ctx is not self.ctx:
             _refuse("the batch belongs to another context")
 
     def append(self, layer: int, batch: PagedBatch, rope: Rope | None, x: torch.Tensor, heads: int, q_out: torch.Tensor, positions: torch.Tensor | None = None) -> None:
         """Rows of x [rows, (heads + 2 kv_heads) * dim] (queries, keys, values): turned queries to q_out [rows, heads * dim], turned keys and the
         values to the layer's pages.  ``positions`` [rows]: turn by these instead of the positions in the sequences."""
-        c, ctx = self._layer(layer), self.ctx
-        self._same(batch)
-        ldx = _rows(x, "x", (torch.float32, torch.bfloat16), batch.rows, (heads + 2 * self.kv_heads) * self.dim, ctx)
-        ldq = _rows(q_out, "q_out", (torch.float32, torch.bfloat16), batch.rows, heads * self.dim, ctx)
+        ctx, rows = self.ctx, batch.rows
+        self._check(layer, batch)
+        ldx = _rows(x, "x", _IN, rows, (heads + 2 * self.kv_heads) * self.dim, ctx)
+        ldq = _rows(q_out, "q_out", _IN, rows, heads * self.dim, ctx)
         if positions is not None:
             _on_device(positions, "positions", _INT, ctx)
             if positions.numel() < batch.rows:
                 _refuse(f"positions must hold {batch.rows} numbers")
-        if rope is not None and rope.freq.device.index != ctx.device:
+        if rope is not None and rope.device != ctx.device:
             _refuse(f"freq must be on cuda:{ctx.device}")
-        ctx._check(ctx._lib.hf2q_cuda_pages_append(ctx._h, ctx._stream(), C.byref(c), C.byref(batch.struct), None if rope is None else C.byref(rope.struct(positions)),
-                                                   x.data_ptr(), _TORCH_DT[x.dtype], ldx, heads, q_out.data_ptr(), _TORCH_DT[q_out.dtype], ldq))
+        turn = None if rope is None else rope.ref if positions is None else C.byref(rope.struct(positions))
+        rc = self._append(ctx._h, ctx._stream(), self._refs[layer], batch.ref, turn, x.data_ptr(), _TORCH_DT[x.dtype], ldx, heads, q_out.data_ptr(), _TORCH_DT[q_out.dtype], ldq)
+        if rc:
+            ctx._check(rc)
 
     def attend(self, layer: int, batch: PagedBatch, q: torch.Tensor, heads: int, out: torch.Tensor, scale: float | None = None, window: int = 0, sinks: int = 0) -> None:
         """out [rows, heads * dim] = attention of q's rows over their sequences (``scale`` None: dim^-1/2; ``window`` 0: all positions before)."""
-        c, ctx = self._layer(layer), self.ctx
-        self._same(batch)
-        ldq = _rows(q, "q", (torch.float32, torch.bfloat16), batch.rows, heads * self.dim, ctx)
-        ldo = _rows(out, "out", (torch.float32, torch.bfloat16, torch.float16), batch.rows, heads * self.dim, ctx)
+        ctx, rows, width = self.ctx, batch.rows, heads * self.dim
+        self._check(layer, batch)
+        ldq, ldo = _rows(q, "q", _IN, rows, width, ctx), _rows(out, "out", _OUT, rows, width, ctx)
         if window < 0 or sinks < 0:
             _refuse("window and sinks are not negative")
-        scratch = batch.scratch(c, heads, window, sinks)
-        ctx._check(ctx._lib.hf2q_cuda_pages_attend(ctx._h, ctx._stream(), C.byref(c), C.byref(batch.struct), q.data_ptr(), _TORCH_DT[q.dtype], ldq, heads,
-                                                   self.dim ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(), _TORCH_DT[out.dtype], ldo,
-                                                   scratch.data_ptr(), scratch.numel()))
+        scratch = batch.scratch(self._structs[layer], heads, window, sinks)
+        rc = self._attend(ctx._h, ctx._stream(), self._refs[layer], batch.ref, q.data_ptr(), _TORCH_DT[q.dtype], ldq, heads, self._scale if scale is None else scale, window, sinks,
+                          out.data_ptr(), _TORCH_DT[out.dtype], ldo, scratch.data_ptr(), scratch.numel())
+        if rc:
+            ctx._check(rc)
 
     def _move(self, entry: str, src: torch.Tensor, dst: torch.Tensor) -> None:
         ctx = self.ctx
@@ -182,7 +190,7 @@ class PagedCache:
         _on_device(dst, "dst", _INT, ctx)
         if src.numel() != dst.numel():
             _refuse("src and dst name as many places")
-        ctx._check(getattr(ctx._lib, entry)(ctx._h, ctx._stream(), C.byref(self._structs[0]), self.layers, src.data_ptr(), dst.data_ptr(), src.numel()))
+        ctx._check(getattr(ctx._lib, entry)(ctx._h, ctx._stream(), self._refs[0], self.layers, src.data_ptr(), dst.data_ptr(), src.numel()))
 
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Pages src[i] -> dst[i] of all layers; no destination is a source or named twice."""
