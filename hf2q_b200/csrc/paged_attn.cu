@@ -59,7 +59,10 @@ cudaError_t launch_join(const AttendCall& a) {
 }
 
 // How a call is laid out, from the bounds that the host knows.
-constexpr uint64_t STEP_UNITS = 32;          // rows of a sequence (tokens times heads of a group) that the step kernel takes
+// Rows of a sequence (tokens times heads of a group) that the step kernel takes: one tile of 16; and up to four over short contexts, where the
+// other kernel's start is what takes long (us, step / tiles: 32 rows of 8000 positions 30.2 / 27.6, 64 rows 36.2 / 27.7; 48 rows of 300 positions
+// 14.3 / 17.2, 64 rows of 60 10.3 / 13.2).
+constexpr uint64_t STEP_UNITS = 16, STEP_SHORT_UNITS = 64, STEP_SHORT = 1024;
 struct Plan {
     bool step;
     uint32_t chunk, chunks;
@@ -68,7 +71,7 @@ struct Plan {
 Plan plan_of(const hf2q_pages& c, const hf2q_page_batch& b, uint32_t heads, uint32_t window, uint32_t sinks, int sms) {
     Plan p{};
     const uint64_t group = heads / c.kv_heads, units = b.max_new * group;
-    p.step = units <= STEP_UNITS;
+    p.step = units <= STEP_UNITS || (units <= STEP_SHORT_UNITS && b.max_length <= STEP_SHORT);
     const uint64_t rows = units <= 8 ? 8 : p.step ? 16 : 2 * (128 / group) * group;
     // most positions that a tile goes through, and tiles as if every sequence that can have rows had the most
     const uint64_t ceil128 = (b.max_length + 127ull) / 128 * 128, seqs = std::min(b.seqs, b.rows);

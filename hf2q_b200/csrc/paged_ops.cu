@@ -80,7 +80,7 @@ template <int V> __device__ __forceinline__ void store_some(__nv_bfloat16* p, bo
 }
 
 // A CTA per row of the batch, or a share of its heads where the rows alone would leave SMs idle; a warp per head, dim / 32 elements a
-// lane.  Partners of a pair meet in shared memory, which serves both layouts and any rot_dim.
+// lane, the next head's load under way.
 constexpr uint32_t AP_WARPS = 8;
 template <int DIM, typename X, typename Q, bool CODES>
 __global__ void __launch_bounds__(AP_WARPS * 32) append_kernel(Pool c, Batch b, Turn turn, AppendShape sh, const X* x, Q* q_out, uint32_t* status) {
@@ -103,33 +103,56 @@ __global__ void __launch_bounds__(AP_WARPS * 32) append_kernel(Pool c, Batch b, 
     if (bad && threadIdx.x == 0) atomicOr(status, STATUS_BAD_PAGE);
     if (bad) return;
     const uint32_t half = turn.rot / 2;
+    const X* row = x + static_cast<size_t>(t) * sh.ldx;
+    const uint32_t h0 = warp + blockIdx.y * AP_WARPS, step = gridDim.y * AP_WARPS;
+    float e[V], later[V];                                                // a head, and the next one on its way
+    if (h0 < all) load_some<V>(row + static_cast<size_t>(h0) * DIM + V * lane, sh.wide_x, later);
     if (threadIdx.x < half) {
         double sn, co;
         sincos(static_cast<double>(turn.pos ? turn.pos[t] : pos) * static_cast<double>(turn.freq[threadIdx.x]), &sn, &co);
         cs[threadIdx.x] = make_float2(static_cast<float>(co) * turn.factor, static_cast<float>(sn) * turn.factor);
     }
     __syncthreads();
-    const X* row = x + static_cast<size_t>(t) * sh.ldx;
-    const uint32_t in_page = pos & (c.size() - 1);
-    for (uint32_t h = warp + blockIdx.y * AP_WARPS; h < all; h += gridDim.y * AP_WARPS) {
-        float e[V];
-        load_some<V>(row + static_cast<size_t>(h) * DIM + V * lane, sh.wide_x, e);
-        if (half && h < sh.heads + c.kv_heads) {
-            float* mine = head[warp];
-            store_some<V>(mine + V * lane, true, e);
-            __syncwarp();
+    // cosine and sine of this lane's elements, the same for all heads; the sine with the sign that it has there
+    float co[V], si[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const uint32_t i = V * lane + j;
-                if (i < turn.rot) {
-                    const bool second = turn.halves ? i >= half : (i & 1);
-                    const uint32_t pair = turn.halves ? (second ? i - half : i) : i >> 1;
-                    const float other = mine[turn.halves ? (second ? i - half : i + half) : (i ^ 1)];
-                    const float2 w = cs[pair];
-                    e[j] = second ? __fadd_rn(__fmul_rn(other, w.y), __fmul_rn(e[j], w.x)) : __fsub_rn(__fmul_rn(e[j], w.x), __fmul_rn(other, w.y));
+    for (int j = 0; j < V; ++j) {
+        const uint32_t i = V * lane + j;
+        const bool second = turn.halves ? i >= half : (i & 1);
+        const float2 w = i < turn.rot ? cs[turn.halves ? (second ? i - half : i) : i >> 1] : make_float2(1.f, 0.f);
+        co[j] = w.x;
+        si[j] = second ? w.y : -w.y;
+    }
+    // halves: the partner is the same element of another lane, or (halves that end inside a lane's elements) comes through shared memory
+    const bool by_lane = half % V == 0;
+    const uint32_t partner = V * lane < half ? lane + half / V : lane - half / V;
+    const uint32_t in_page = pos & (c.size() - 1);
+    for (uint32_t h = h0; h < all; h += step) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) e[j] = later[j];
+        if (h + step < all) load_some<V>(row + static_cast<size_t>(h + step) * DIM + V * lane, sh.wide_x, later);
+        if (half && h < sh.heads + c.kv_heads) {
+            float other[V];
+            if (!turn.halves) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) other[j] = e[j ^ 1];
+            } else if (by_lane) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) other[j] = __shfl_sync(0xffffffffu, e[j], partner & 31);
+            } else {
+                float* mine = head[warp];
+                store_some<V>(mine + V * lane, true, e);
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const uint32_t i = V * lane + j;
+                    other[j] = i < turn.rot ? mine[i >= half ? i - half : i + half] : 0.f;
                 }
+                __syncwarp();
             }
-            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (V * lane + j < turn.rot) e[j] = __fadd_rn(__fmul_rn(e[j], co[j]), __fmul_rn(other[j], si[j]));
         }
         if (h < sh.heads) {
             store_some<V>(q_out + static_cast<size_t>(t) * sh.ldq + static_cast<size_t>(h) * DIM + V * lane, sh.wide_q, e);
