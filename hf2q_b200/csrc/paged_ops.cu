@@ -96,12 +96,12 @@ __global__ void __launch_bounds__(AP_WARPS * 32) append_kernel(Pool c, Batch b, 
         return;
     }
     const Span span = span_of(b, c.shift, s);
-    const bool held = t - span.row0 < span.rows && span.length + (t - span.row0) >= span.rows;       // it has a position
+    const bool held = t - span.row0 < span.rows && span.length + (t - span.row0) >= span.rows;       // it has a position (padding in front has none)
     const uint32_t pos = held ? span.length - span.rows + (t - span.row0) : 0;
-    bool bad = span.bad || !held;
+    bool bad = span.bad;
     const uint32_t page = held ? page_of(c, b, s, pos, bad) : 0;
     if (bad && threadIdx.x == 0) atomicOr(status, STATUS_BAD_PAGE);
-    if (bad) return;
+    if (bad || !held) return;
     const uint32_t half = turn.rot / 2;
     const X* row = x + static_cast<size_t>(t) * sh.ldx;
     const uint32_t h0 = warp + blockIdx.y * AP_WARPS, step = gridDim.y * AP_WARPS;

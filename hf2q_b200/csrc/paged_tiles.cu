@@ -165,9 +165,11 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
     __shared__ uint32_t tmem_slot;
     const uint32_t kvh = blockIdx.x % c.kv_heads, chunk = blockIdx.y, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     uint32_t seq = 0, tok0 = 0;
+    if (blockIdx.x == 0 && chunk == 0)                                    // (a sequence that does not fit may have no tile to say so)
+        for (uint32_t s = threadIdx.x; s < b.seqs; s += THREADS)
+            if (span_of(b, c.shift, s).bad) atomicOr(status, STATUS_BAD_PAGE);
     if (!find_tile(b, c.shift, 2 * sh.tokens, (gridDim.x - 1 - blockIdx.x) / c.kv_heads, seq, tok0)) return;      // (the tiles with the most positions first)
     const Span span = span_of(b, c.shift, seq);
-    if (span.bad && threadIdx.x == 0) atomicOr(status, STATUS_BAD_PAGE);
     const uint32_t end_tok = min(tok0 + 2 * sh.tokens, span.rows), tiles = end_tok - tok0 > sh.tokens ? 2 : 1;
     const uint32_t lost = span.rows > span.length ? span.rows - span.length : 0;      // rows in front of position 0: they see nothing
     const uint32_t before = span.length - span.rows;                      // position of token 0 (wraps where rows are lost)

@@ -937,8 +937,9 @@ typedef struct hf2q_pages {
 /* The rows of one call.  Sequence s owns rows start[s] .. start[s + 1] - 1 (possibly none) and holds length[s] positions, the new ones
  * included: its rows are the last of them, in order.  Position p is row p % page of page table[s][p / page].  The arrays are read on
  * the device, so that a captured call can be replayed on other values; the call itself is laid out for `rows` rows in all, at most
- * max_new rows and max_length positions of a sequence.  Rows behind start[seqs] are left as they were.  What does not fit (a
- * page number >= pages, a length above max_length or the table, more than max_new rows, a row before position 0, starts that run
+ * max_new rows and max_length positions of a sequence.  Rows behind start[seqs] are left as they were.  With more rows than positions
+ * the first rows are padding: they are not appended and see nothing (their attention is zero).  What does not fit (a
+ * page number >= pages, a length above max_length or the table, more than max_new rows, starts that run
  * backwards or past `rows`) touches no memory outside the arrays and is reported by hf2q_cuda_check_status; the outputs of the
  * sequences that it concerns mean nothing. */
 typedef struct hf2q_page_batch {
@@ -962,7 +963,7 @@ HF2Q_API int32_t hf2q_cuda_pages_append(hf2q_ctx* ctx, void* stream, const hf2q_
                                         uint32_t heads, void* q_out, uint32_t q_dtype, uint32_t ldq);
 /* Attention of every row over its sequence's positions (appended before): out[row][heads][dim] = softmax(q . k * scale) . v; query
  * head h reads KV head h / (heads / kv_heads).  Position j is visible to i when j <= i and, with window > 0, i - j < window or
- * j < sinks.  A row that sees nothing is zero; what a row does not see has no part in it, infinities and NaN included.  q f32 or
+ * j < sinks.  What a row does not see has no part in it, infinities and NaN included.  q f32 or
  * bf16, out f32, bf16 or f16 (beyond the f16 range clipped and noted in the status).  Codes are multiplied as exact f16 numbers
  * with q in f16 (clipped and noted), bf16 keys with q in bf16; probabilities are rounded to the same type, sums are f32.
  * scratch: 256-byte aligned, of hf2q_cuda_pages_attend_scratch_bytes; its contents need not be kept. */
