@@ -8,19 +8,19 @@ import sys
 from pathlib import Path
 
 
-def _model(args, max_seq: int, n_slots: int):
+def _model(args, max_seq: int, n_slots: int, pages: int | None = None):
     from . import build
     build.build()
     import torch
     from . import ops, registry
     ctx = ops.GpuContext(0)
-    return ctx, registry.load_model(ctx, args.model, dtype=getattr(torch, args.dtype), max_seq=max_seq, n_slots=n_slots)
+    return ctx, registry.load_model(ctx, args.model, dtype=getattr(torch, args.dtype), max_seq=max_seq, n_slots=n_slots, pages=pages)
 
 
 def generate(args) -> int:
     from .engine import Engine
     prompts = [[int(t) for t in p.split(",")] for p in args.prompt]
-    ctx, model = _model(args, args.max_seq, min(len(prompts), args.slots))
+    ctx, model = _model(args, args.max_seq, min(len(prompts), args.slots), args.pages)
     for ids in Engine(model).generate(prompts, args.new):
         print(json.dumps(ids))
     ctx.check_status()
@@ -53,6 +53,7 @@ def main(argv=None) -> int:
     g.add_argument("--new", type=int, default=16, help="tokens to generate per prompt")
     g.add_argument("--max-seq", type=int, default=32768)
     g.add_argument("--slots", type=int, default=4, help="sequences held at a time")
+    g.add_argument("--pages", type=int, help="keep the sequences of a .gguf model in a pool of this many pages of 64 tokens, --slots of them at a time")
     g.set_defaults(run=generate)
     t = sub.add_parser("trace", help="replay token ids read from standard input, step by step")
     t.add_argument("--out", required=True, help="folder for <step>.f32")

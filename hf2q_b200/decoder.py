@@ -311,15 +311,7 @@ class LlamaDecoder(GreedyDecoder):
         self.dev = dev
         c = cfg
         self.qkv_cols = c.q_rows + 2 * c.kv_rows
-        # the 8-bit KV cache: one pair of (codes, scales) for K and for V per layer
-        self.kv_bufs, self.kv = [], []
-        for _ in range(c.n_layers):
-            kc = torch.zeros((c.n_kv_heads, c.max_seq, c.head_dim), dtype=torch.int8, device=dev)
-            ks = torch.zeros((c.n_kv_heads, c.max_seq), dtype=torch.float32, device=dev)
-            vc = torch.zeros_like(kc)
-            vs = torch.zeros_like(ks)
-            self.kv_bufs.append((kc, ks, vc, vs))
-            self.kv.append(_KvCache(kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), c.n_kv_heads, c.head_dim, c.max_seq))
+        self._allocate_cache()
         # device-resident loop state
         self.pos = torch.zeros(1, dtype=torch.int32, device=dev)          # position of the token being processed
         self.tok = torch.zeros(1, dtype=torch.int32, device=dev)          # its id (written by the arg-max kernel)
@@ -351,10 +343,27 @@ class LlamaDecoder(GreedyDecoder):
             if not ops.quantized_matmul_swiglu_supported(ctx, 1, lw.gate, torch.float32):
                 raise ops.Hf2qError(_lib.ERR_INVALID_ARGUMENT, "gate/up shape does not fit the fused SwiGLU launch")
 
+    def _allocate_cache(self) -> None:
+        """The 8-bit KV cache: one pair of (codes, scales) for K and for V per layer."""
+        c, dev = self.cfg, self.dev
+        self.kv_bufs, self.kv = [], []
+        for _ in range(c.n_layers):
+            kc = torch.zeros((c.n_kv_heads, c.max_seq, c.head_dim), dtype=torch.int8, device=dev)
+            ks = torch.zeros((c.n_kv_heads, c.max_seq), dtype=torch.float32, device=dev)
+            vc = torch.zeros_like(kc)
+            vs = torch.zeros_like(ks)
+            self.kv_bufs.append((kc, ks, vc, vs))
+            self.kv.append(_KvCache(kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), c.n_kv_heads, c.head_dim, c.max_seq))
+
     @classmethod
     def from_gguf(cls, ctx: ops.GpuContext, path, max_seq: int = 32768, prefill_chunk: int = 2048) -> "LlamaDecoder":
         """Loads a GGUF file with the ``llama`` key prefix and tensor names (block bytes unchanged; an absent
         output.weight means the tied embedding)."""
+        return cls._load_gguf(ctx, path, max_seq, prefill_chunk, cls)
+
+    @staticmethod
+    def _load_gguf(ctx: ops.GpuContext, path, max_seq: int, prefill_chunk: int, make):
+        """``make(ctx, cfg, weights, prefill_chunk)`` of what the file holds."""
         from .gguf import GgufFile
         with GgufFile(path) as g:
             md = lambda k, default=None: g.metadata.get("llama." + k, default)
@@ -384,7 +393,7 @@ class LlamaDecoder(GreedyDecoder):
                                            weight(p + "attn_output.weight"), vec(p + "ffn_norm.weight"), weight(p + "ffn_gate.weight"),
                                            weight(p + "ffn_up.weight"), weight(p + "ffn_down.weight")))
             out = "output.weight" if "output.weight" in g.tensors else "token_embd.weight"
-            return cls(ctx, cfg, ModelWeights(weight("token_embd.weight"), layers, vec("output_norm.weight"), weight(out)), prefill_chunk)
+            return make(ctx, cfg, ModelWeights(weight("token_embd.weight"), layers, vec("output_norm.weight"), weight(out)), prefill_chunk)
 
     # ---- thin wrappers over the C ABI (current stream) -----------------------------------------
     def _s(self):
@@ -425,6 +434,29 @@ class LlamaDecoder(GreedyDecoder):
             ops.quantized_matmul_ggml(self.ctx, inp, weight, self.tmp, weight.matmul_params(1))
             self.ctx._check(self.lib.hf2q_cuda_add(self.ctx._h, self._s(), self.x.data_ptr(), self.tmp.data_ptr(), self.x.numel()))
 
+    # ---- attention: the new tokens' keys and values to the cache, then over it ------------------
+    def _attend_step(self, i: int) -> None:
+        """Layer i of a decode step: self.qkv at position self.pos -> self.att."""
+        c, ctx, lib = self.cfg, self.ctx, self.lib
+        if self.fused_attention:      # rotary + KV append + split attention + merge: one launch
+            ctx._check(lib.hf2q_cuda_attn_decode_fused(ctx._h, self._s(), self.qkv.data_ptr(), c.n_heads, c.rope_theta, C.byref(self.kv[i]),
+                                                       self.pos.data_ptr(), self.att.data_ptr(), ops.DT_F32, self.att_scratch.data_ptr(),
+                                                       self.att_scratch.numel()))
+        else:
+            self._rope_append(self.qkv, 1, i)
+            ctx._check(lib.hf2q_cuda_attn_decode(ctx._h, self._s(), self.qkv.data_ptr(), c.n_heads, C.byref(self.kv[i]), self.pos.data_ptr(),
+                                                 self.att.data_ptr(), ops.DT_F32, self.att_scratch.data_ptr(), self.att_scratch.numel()))
+
+    def _attend_portion(self, i: int, qkv, m: int, p0: int, att) -> None:
+        """Layer i of a portion of m tokens from position p0 on: qkv -> att, f32 or an f16 panel."""
+        c, ctx, lib = self.cfg, self.ctx, self.lib
+        self._rope_append(qkv, m, i)
+        if att.dtype == torch.float16:
+            ctx._check(lib.hf2q_cuda_attn_prefill_panel(ctx._h, self._s(), qkv.data_ptr(), m, c.n_heads, C.byref(self.kv[i]), p0, att.data_ptr()))
+        else:
+            ctx._check(lib.hf2q_cuda_attn_prefill(ctx._h, self._s(), qkv.data_ptr(), m, c.n_heads, C.byref(self.kv[i]), p0,
+                                                  att.data_ptr(), ops.DT_F32))
+
     # ---- one decode step: token self.tok at position self.pos -> next token, position + 1 -------
     def decode_step(self) -> None:
         c, ctx, lib = self.cfg, self.ctx, self.lib
@@ -436,14 +468,7 @@ class LlamaDecoder(GreedyDecoder):
             else:
                 self._rms(self.x, None, lw.attn_norm, self.xn, 1)
                 ops.quantized_matmul_segments(ctx, self.xn, self._qkv_segments(lw), self.qkv, 1)
-            if self.fused_attention:      # rotary + KV append + split attention + merge: one launch
-                ctx._check(lib.hf2q_cuda_attn_decode_fused(ctx._h, self._s(), self.qkv.data_ptr(), c.n_heads, c.rope_theta, C.byref(self.kv[i]),
-                                                           self.pos.data_ptr(), self.att.data_ptr(), ops.DT_F32, self.att_scratch.data_ptr(),
-                                                           self.att_scratch.numel()))
-            else:
-                self._rope_append(self.qkv, 1, i)
-                ctx._check(lib.hf2q_cuda_attn_decode(ctx._h, self._s(), self.qkv.data_ptr(), c.n_heads, C.byref(self.kv[i]), self.pos.data_ptr(),
-                                                     self.att.data_ptr(), ops.DT_F32, self.att_scratch.data_ptr(), self.att_scratch.numel()))
+            self._attend_step(i)
             self._matmul_add(self.att, lw.wo)                                               # x += O(att)
             if fn:
                 ops.quantized_matmul_swiglu(ctx, self.x, lw.gate, lw.up, self.act, 1, norm_weight=lw.ffn_norm, norm_eps=c.rms_eps)
@@ -532,8 +557,7 @@ class LlamaDecoder(GreedyDecoder):
                 if panels:
                     self._rms_panel(x, lw.attn_norm, xn, m)
                     self._matmul_panel(xn, self._qkv_segments(lw), qkv, m)
-                    self._rope_append(qkv, m, i)
-                    ctx._check(lib.hf2q_cuda_attn_prefill_panel(ctx._h, self._s(), qkv.data_ptr(), m, c.n_heads, C.byref(self.kv[i]), p0, att.data_ptr()))
+                    self._attend_portion(i, qkv, m, p0, att)
                     self._matmul_panel(att, [lw.wo], x, m, x)
                     self._rms_panel(x, lw.ffn_norm, xn, m)
                     ctx._check(lib.hf2q_cuda_qmatmul_swiglu_panel(ctx._h, self._s(), xn.data_ptr(), ops.DT_F16, lw.gate.ptr, lw.up.ptr, g.data_ptr(), m, lw.gate.rows,
@@ -542,9 +566,7 @@ class LlamaDecoder(GreedyDecoder):
                     continue
                 self._rms(x, delta, lw.attn_norm, xn, m)                                   # x += previous layer's FFN output (unfused form)
                 ops.quantized_matmul_segments(ctx, xn, self._qkv_segments(lw), qkv, m)
-                self._rope_append(qkv, m, i)
-                ctx._check(lib.hf2q_cuda_attn_prefill(ctx._h, self._s(), qkv.data_ptr(), m, c.n_heads, C.byref(self.kv[i]), p0,
-                                                      att.data_ptr(), ops.DT_F32))
+                self._attend_portion(i, qkv, m, p0, att)
                 # the residual stream is updated in the epilogue of the O and down products where the shape allows
                 if self.fused_prefill and ops.quantized_matmul_add_supported(ctx, lw.wo, att.dtype, m):
                     ops.quantized_matmul_add(ctx, att, lw.wo, x, x, m)

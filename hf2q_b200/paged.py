@@ -7,6 +7,7 @@ which page: it hands pages out, shares them between branches of a sequence, and 
 from __future__ import annotations
 
 import ctypes as C
+import heapq
 import math
 
 import torch
@@ -135,9 +136,9 @@ class PagedCache:
         self.ctx, self.k, self.v, self.k_scale, self.v_scale = ctx, k, v, k_scale, v_scale
         self.layers, self.pages, self.kv_heads, self.page, self.dim = k.shape
         at = lambda t, layer: None if t is None else t[layer].data_ptr()
-        self._structs = [_Pages(at(k, i), at(v, i), at(k_scale, i), at(v_scale, i), self.pages, self.page, self.kv_heads, self.dim, DT_I8 if codes else DT_BF16)
+        self.structs = [_Pages(at(k, i), at(v, i), at(k_scale, i), at(v_scale, i), self.pages, self.page, self.kv_heads, self.dim, DT_I8 if codes else DT_BF16)
                          for i in range(self.layers)]
-        self._refs, self._scale = [C.byref(s) for s in self._structs], self.dim ** -0.5
+        self._refs, self._scale = [C.byref(s) for s in self.structs], self.dim ** -0.5
         self._append, self._attend = ctx._lib.hf2q_cuda_pages_append, ctx._lib.hf2q_cuda_pages_attend
 
     @classmethod
@@ -178,7 +179,7 @@ class PagedCache:
         ldq, ldo = _rows(q, "q", _IN, rows, width, ctx), _rows(out, "out", _OUT, rows, width, ctx)
         if window < 0 or sinks < 0:
             _refuse("window and sinks are not negative")
-        scratch = batch.scratch(self._structs[layer], heads, window, sinks)
+        scratch = batch.scratch(self.structs[layer], heads, window, sinks)
         rc = self._attend(ctx._h, ctx._stream(), self._refs[layer], batch.ref, q.data_ptr(), _TORCH_DT[q.dtype], ldq, heads, self._scale if scale is None else scale, window, sinks,
                           out.data_ptr(), _TORCH_DT[out.dtype], ldo, scratch.data_ptr(), scratch.numel())
         if rc:
@@ -199,3 +200,158 @@ class PagedCache:
     def copy_rows(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Rows src[i] -> dst[i] of all layers (row r of page g is g * page + r); no destination is a source or named twice."""
         self._move("hf2q_cuda_pages_copy_rows", src, dst)
+
+
+class PagePool:
+    """Which sequence owns which pages of a cache, kept on the host: pages are handed out lowest number first, branches of a sequence share
+    them, and a shared page is copied before one of its owners writes into it.
+
+    ``table`` [seqs, pages of max_length] and ``length`` [seqs] on the device follow the books, in the order of the current stream, for
+    ``PagedBatch`` to read."""
+
+    def __init__(self, cache: PagedCache, seqs: int, max_length: int):
+        if seqs < 1 or max_length < 1:
+            _refuse("a pool serves 1 sequence or more, of 1 position or more")
+        self.cache, self.seqs, self.max_length = cache, seqs, max_length
+        dev = cache.k.device
+        self.table = torch.full((seqs, -(-max_length // cache.page)), -1, dtype=torch.int32, device=dev)
+        self.length = torch.zeros(seqs, dtype=torch.int32, device=dev)
+        self._free, self._refs = list(range(cache.pages)), [0] * cache.pages             # (a heap)
+        self._pages: list = [None] * seqs                                                # page numbers of an open sequence
+        self._lengths = [0] * seqs
+
+    # ---- what the books say
+    @property
+    def n_free_pages(self) -> int:
+        return len(self._free)
+
+    def pages_of(self, seq: int) -> list:
+        return list(self._own(seq))
+
+    def length_of(self, seq: int) -> int:
+        self._own(seq)
+        return self._lengths[seq]
+
+    def _own(self, seq: int) -> list:
+        if not 0 <= seq < self.seqs or self._pages[seq] is None:
+            raise RuntimeError(f"sequence {seq} is not in use")
+        return self._pages[seq]
+
+    def _vacant(self) -> int:
+        for s, p in enumerate(self._pages):
+            if p is None:
+                return s
+        raise RuntimeError("no free sequence slot")
+
+    def _take(self, n: int) -> list:
+        if n > len(self._free):
+            raise RuntimeError(f"no free page ({n} wanted, {len(self._free)} of {self.cache.pages} free)")
+        out = [heapq.heappop(self._free) for _ in range(n)]
+        for p in out:
+            self._refs[p] = 1
+        return out
+
+    def _drop(self, pages) -> None:
+        for p in pages:
+            self._refs[p] -= 1
+            if self._refs[p] == 0:
+                heapq.heappush(self._free, p)
+
+    def _numbers(self, values) -> torch.Tensor:
+        return torch.tensor(values, dtype=torch.int32).to(self.table.device)
+
+    def _publish(self, seq: int) -> None:
+        """The device's row and length; a place without a page holds -1, which the entries report and skip."""
+        pages = self._pages[seq] or []
+        if pages:
+            self.table[seq, :len(pages)] = self._numbers(pages)
+        self.table[seq, len(pages):].fill_(-1)
+        self.length[seq:seq + 1].fill_(self._lengths[seq])
+
+    # ---- sequences
+    def open(self) -> int:
+        """A new sequence without positions."""
+        seq = self._vacant()
+        self._pages[seq], self._lengths[seq] = [], 0
+        self._publish(seq)
+        return seq
+
+    def close(self, seq: int) -> None:
+        """Gives the sequence's pages back, as far as no branch shares them."""
+        self._drop(self._own(seq))
+        self._pages[seq], self._lengths[seq] = None, 0
+        self._publish(seq)
+
+    def reserve(self, seq: int, n: int) -> None:
+        """Pages of its own for the sequence's next n positions (which ``advance`` then counts)."""
+        pages, size, have = self._own(seq), self.cache.page, self._lengths[seq]
+        if n < 0 or have + n > self.max_length:
+            _refuse(f"{n} positions after {have}: the pool holds sequences of up to {self.max_length}")
+        if n == 0:
+            return
+        first = have // size
+        shared = [i for i in range(first, len(pages)) if self._refs[pages[i]] > 1]       # pages that will be written into
+        new = self._take(len(shared) + max(0, -(-(have + n) // size) - len(pages)))
+        if shared:
+            used = [i for i in shared if i * size < have]                                # only the one that is partly filled holds anything
+            if used:
+                self.cache.copy_pages(self._numbers([pages[i] for i in used]), self._numbers(new[:len(used)]))
+            old = [pages[i] for i in shared]
+            for i, p in zip(shared, new):
+                pages[i] = p
+            self._drop(old)
+        pages += new[len(shared):]
+        if new:
+            self.table[seq, first:len(pages)] = self._numbers(pages[first:])
+
+    def advance(self, seq: int, n: int) -> None:
+        """The sequence has n more positions, in pages that ``reserve`` gave it."""
+        pages, total = self._own(seq), self._lengths[seq] + n
+        if n < 0 or total > len(pages) * self.cache.page:
+            _refuse(f"{n} positions were not reserved")
+        self._lengths[seq] = total
+        self.length[seq:seq + 1].fill_(total)
+
+    def fork(self, seq: int) -> int:
+        """A branch with the same positions: it shares the pages until one of the two writes."""
+        pages = self._own(seq)
+        branch = self._vacant()
+        keep = pages[:-(-self._lengths[seq] // self.cache.page)]
+        for p in keep:
+            self._refs[p] += 1
+        self._pages[branch], self._lengths[branch] = list(keep), self._lengths[seq]
+        self._publish(branch)
+        return branch
+
+    def compact(self, seq: int, keep) -> None:
+        """Keeps the given positions (ascending) and packs them; the others are forgotten.  Keys stay turned as they are."""
+        pages, size = self._own(seq), self.cache.page
+        keep = [int(p) for p in keep]
+        if any(a >= b for a, b in zip(keep, keep[1:])) or (keep and (keep[0] < 0 or keep[-1] >= self._lengths[seq])):
+            _refuse("positions to keep are ascending and among the sequence's own")
+        same = 0                                                                         # pages at the front that stay as they are
+        while (same + 1) * size <= len(keep) and keep[(same + 1) * size - 1] == (same + 1) * size - 1:
+            same += 1
+        rest = keep[same * size:]
+        new = self._take(-(-len(rest) // size))
+        if rest:
+            self.cache.copy_rows(self._numbers([pages[p // size] * size + p % size for p in rest]), self._numbers([new[i // size] * size + i % size for i in range(len(rest))]))
+        self._drop(pages[same:])
+        self._pages[seq], self._lengths[seq] = pages[:same] + new, len(keep)
+        self._publish(seq)
+
+    def pack(self) -> int:
+        """Moves pages to the lowest numbers; returns how many pages, from the front, are in use."""
+        used = sorted(p for p, n in enumerate(self._refs) if n)
+        moves = [(p, i) for p, i in zip(reversed([p for p in used if p >= len(used)]), [p for p in range(len(used)) if self._refs[p] == 0])]
+        if moves:
+            self.cache.copy_pages(self._numbers([a for a, _ in moves]), self._numbers([b for _, b in moves]))
+            to = dict(moves)
+            for a, b in moves:
+                self._refs[b], self._refs[a] = self._refs[a], 0
+            for seq, pages in enumerate(self._pages):
+                if pages is not None and any(p in to for p in pages):
+                    self._pages[seq] = [to.get(p, p) for p in pages]
+                    self._publish(seq)
+            self._free = list(range(len(used), self.cache.pages))
+        return len(used)

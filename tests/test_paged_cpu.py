@@ -116,3 +116,122 @@ def test_null_contexts_are_refused():
     assert lib.hf2q_cuda_pages_append(None, None, None, None, None, None, 0, 0, 0, None, 0, 0) == _lib.ERR_INVALID_ARGUMENT
     assert lib.hf2q_cuda_pages_copy(None, None, None, 1, None, None, 0) == _lib.ERR_INVALID_ARGUMENT
     assert lib.hf2q_cuda_pages_copy_rows(None, None, None, 1, None, None, 0) == _lib.ERR_INVALID_ARGUMENT
+
+
+class Contents:
+    """Stands in for a cache: one number a row, on the CPU."""
+
+    def __init__(self, pages, page):
+        self.pages, self.page, self.k = pages, page, torch.zeros(())
+        self.rows = [-1] * (pages * page)
+
+    def copy_rows(self, src, dst):
+        src, dst = src.tolist(), dst.tolist()
+        assert len(set(dst)) == len(dst) and not set(src) & set(dst)
+        for a, b in zip(src, dst):
+            self.rows[b] = self.rows[a]
+
+    def copy_pages(self, src, dst):
+        at = lambda t: (t[:, None] * self.page + torch.arange(self.page)).view(-1)
+        self.copy_rows(at(src), at(dst))
+
+
+def write(cache, pool, seq, values):
+    pool.reserve(seq, len(values))
+    pages, at = pool.pages_of(seq), pool.length_of(seq)
+    for i, v in enumerate(values, at):
+        cache.rows[pages[i // cache.page] * cache.page + i % cache.page] = v
+    pool.advance(seq, len(values))
+
+
+def same(cache, pool, want):
+    used = set()
+    for seq in range(pool.seqs):
+        row = pool.table[seq].tolist()
+        if seq not in want:
+            assert row == [-1] * len(row) and int(pool.length[seq]) == 0
+            continue
+        pages = pool.pages_of(seq)
+        used |= set(pages)
+        assert len(set(pages)) == len(pages) and row == pages + [-1] * (len(row) - len(pages))
+        assert int(pool.length[seq]) == pool.length_of(seq) == len(want[seq])
+        assert [cache.rows[pages[i // cache.page] * cache.page + i % cache.page] for i in range(len(want[seq]))] == want[seq]
+    assert pool.n_free_pages == cache.pages - len(used)
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_the_pool_keeps_every_sequence_through_branches_packing_and_want_of_pages(seed):
+    rnd = random.Random(seed)
+    cache = Contents(rnd.choice([5, 12, 40]), rnd.choice([1, 4, 16]))
+    pool = paged.PagePool(cache, 4, 6 * cache.page + 1)
+    want, mark, refused = {}, 0, 0
+    for _ in range(400):
+        what, seq = rnd.choice(["open", "write", "write", "write", "fork", "compact", "pack", "close"]), rnd.choice(list(want) or [None])
+        if seq is None:
+            what = "open"
+        try:
+            if what == "open":
+                want[pool.open()] = []
+            elif what == "write":
+                n = rnd.randrange(0, 2 * cache.page + 2)
+                if len(want[seq]) + n > pool.max_length:
+                    with pytest.raises(Hf2qError):
+                        pool.reserve(seq, n)
+                    continue
+                write(cache, pool, seq, list(range(mark, mark + n)))
+                want[seq], mark = want[seq] + list(range(mark, mark + n)), mark + n
+            elif what == "fork":
+                want[pool.fork(seq)] = list(want[seq])
+            elif what == "compact":
+                keep = [i for i in range(len(want[seq])) if i < cache.page * rnd.randrange(3) or rnd.random() < 0.6]
+                pool.compact(seq, keep)
+                want[seq] = [want[seq][i] for i in keep]
+            elif what == "pack":
+                assert pool.pack() == cache.pages - pool.n_free_pages
+                assert all(p < cache.pages - pool.n_free_pages for s in want for p in pool.pages_of(s))
+            else:
+                pool.close(seq)
+                del want[seq]
+        except RuntimeError as e:                          # nothing has changed then
+            assert "no free" in str(e)
+            refused += 1
+        same(cache, pool, want)
+    assert refused
+
+
+def test_the_pool_refuses_what_its_books_do_not_allow():
+    pool = paged.PagePool(Contents(4, 4), 2, 16)
+    with pytest.raises(Hf2qError):
+        paged.PagePool(Contents(4, 4), 0, 16)
+    with pytest.raises(RuntimeError, match="not in use"):
+        pool.reserve(0, 1)
+    a = pool.open()
+    for call in (lambda: pool.reserve(a, 17), lambda: pool.reserve(a, -1), lambda: pool.advance(a, 1), lambda: pool.compact(a, [0])):
+        with pytest.raises(Hf2qError):
+            call()
+    pool.reserve(a, 6)
+    with pytest.raises(Hf2qError):
+        pool.advance(a, 9)
+    pool.advance(a, 6)
+    for keep in ([1, 0], [0, 0], [-1], [6]):
+        with pytest.raises(Hf2qError):
+            pool.compact(a, keep)
+    b = pool.fork(a)
+    with pytest.raises(RuntimeError, match="slot"):
+        pool.open()
+    pool.close(a)
+    with pytest.raises(RuntimeError, match="not in use"):
+        pool.close(a)
+    assert pool.length_of(b) == 6 and pool.n_free_pages == 2
+
+
+def test_frequencies():
+    f = paged.rope_frequencies(8, 10000.0)
+    assert torch.equal(f, torch.tensor([1.0, 0.1, 0.01, 0.001]))
+    assert torch.equal(paged.rope_frequencies(8, 10000.0, linear=4.0), torch.tensor([0.25, 0.025, 0.0025, 0.00025]))
+    # wavelengths 6.3, 63, 628 and 6283 against a trained context of 600: more than 4 turns kept, fewer than 1 divided, 600 / 628 = 0.95 of one too
+    g = paged.rope_frequencies(8, 10000.0, bands={"factor": 8.0, "low": 1.0, "high": 4.0, "trained": 600})
+    assert torch.equal(g, torch.tensor([1.0, 0.1, 0.01 / 8, 0.001 / 8]))
+    # 1257 positions: 2 turns at 0.01, a third of the way between low and high
+    g = paged.rope_frequencies(8, 10000.0, bands={"factor": 8.0, "low": 1.0, "high": 4.0, "trained": 400 * 3.141592653589793})
+    torch.testing.assert_close(g[2], torch.tensor(0.01 * (1 / 3 + 2 / 3 / 8)), rtol=2 ** -23, atol=0)
