@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "paged_common.cuh"
 
@@ -16,32 +17,63 @@ namespace hf2q {
 using namespace paged;
 namespace {
 
-// out[row][head] = sum of the parts, each weighted by exp2(its maximum - the largest), over the same sum of their weights.  A warp per row
-// and head; the order is that of the parts.
-constexpr uint32_t JOIN_WARPS = 4;
-template <int DIM, typename OUT>
+// out[row][head] = sum of the parts, each weighted by exp2(its maximum - the largest), over the same sum of their weights.  Bound by the parts'
+// bytes, so a warp asks for eight parts before it adds the first, in the order of the parts.  Up to JOIN_FEW parts a warp per row and head; more are
+// shared by four warps, whose sums are added in the order of the warps.
+constexpr uint32_t JOIN_WARPS = 4, JOIN_FEW = 16;
+template <int DIM, typename OUT, uint32_t SHARE>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(Batch b, uint32_t heads, uint32_t chunks, const float* part, const float* part_ml, OUT* out, uint32_t ldo, uint32_t* status) {
-    constexpr int V = DIM / 32;
+    constexpr int V = DIM / 32, DEEP = 8;
+    using Vec = std::conditional_t<V == 4, float4, float2>;
+    __shared__ float others[SHARE][DIM + 1];
     pdl_trigger();
     pdl_wait();
-    const uint32_t lane = threadIdx.x & 31;
-    const uint64_t unit = static_cast<uint64_t>(blockIdx.x) * JOIN_WARPS + (threadIdx.x >> 5);
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % SHARE;
+    const uint64_t unit = static_cast<uint64_t>(blockIdx.x) * (JOIN_WARPS / SHARE) + warp / SHARE;
     const uint32_t end = min(b.start[b.seqs], b.rows), begin = b.start[0];
-    if (unit >= static_cast<uint64_t>(end) * heads || unit / heads < begin) return;
+    if (unit >= static_cast<uint64_t>(end) * heads || unit / heads < begin) return;       // (all warps that share a row and head)
     const float2* ml = reinterpret_cast<const float2*>(part_ml) + unit * chunks;
     float m_all = -CUDART_INF_F;
     for (uint32_t i = lane; i < chunks; i += 32) m_all = fmaxf(m_all, ml[i].x);
     for (int o = 16; o > 0; o >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, o));
+    const uint32_t mine = (chunks + SHARE - 1) / SHARE, from = min(share * mine, chunks), upto = min(from + mine, chunks);
+    const float* at = part + unit * chunks * DIM + V * lane;
     float acc[V] = {}, sum = 0.f;
-#pragma unroll 4
-    for (uint32_t i = 0; i < chunks; ++i) {
-        const float2 x = ml[i];
-        const float f = part_factor(x.x, x.y, m_all);
-        if (f == 0.f) continue;
-        sum += x.y * f;
-        const float* p = part + (unit * chunks + i) * DIM + V * lane;
+#pragma unroll 1
+    for (uint32_t i0 = from; i0 < upto; i0 += DEEP) {
+        float f[DEEP], l[DEEP];
+        Vec p[DEEP];
 #pragma unroll
-        for (int e = 0; e < V; ++e) acc[e] += p[e] * f;
+        for (int u = 0; u < DEEP; ++u) {
+            const float2 x = i0 + u < upto ? ml[i0 + u] : make_float2(0.f, 0.f);
+            f[u] = part_factor(x.x, x.y, m_all);
+            l[u] = x.y;
+        }
+#pragma unroll
+        for (int u = 0; u < DEEP; ++u) {                                  // (a part that counts for nothing was not written)
+            p[u] = Vec{};
+            if (f[u] != 0.f) p[u] = *reinterpret_cast<const Vec*>(at + static_cast<uint64_t>(i0 + u) * DIM);
+        }
+#pragma unroll
+        for (int u = 0; u < DEEP; ++u) {
+            if (f[u] == 0.f) continue;
+            sum += l[u] * f[u];
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[e] += reinterpret_cast<const float*>(&p[u])[e] * f[u];
+        }
+    }
+    if constexpr (SHARE > 1) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) others[share][V * lane + e] = acc[e];
+        if (lane == 0) others[share][DIM] = sum;
+        __syncthreads();
+        if (share) return;
+#pragma unroll
+        for (uint32_t w = 1; w < SHARE; ++w) {
+            sum += others[w][DIM];
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[e] += others[w][V * lane + e];
+        }
     }
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
     bool clipped = false;
@@ -50,12 +82,18 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(Batch b, uint32_t
     for (int e = 0; e < V; ++e) to[e] = out_value<OUT>(acc[e] * inv, clipped);
     if (clipped) atomicOr(status, STATUS_X_CLIPPED);
 }
+template <int DIM, typename OUT>
+cudaError_t launch_join_out(const AttendCall& a) {
+    const uint64_t units = static_cast<uint64_t>(a.b.rows) * a.heads;
+    const bool few = a.chunks <= JOIN_FEW;
+    const uint64_t ctas = few ? (units + JOIN_WARPS - 1) / JOIN_WARPS : units;
+    if (ctas > 0x7fffffffull) return cudaErrorInvalidValue;
+    return launch_pdl(few ? join_kernel<DIM, OUT, 1> : join_kernel<DIM, OUT, JOIN_WARPS>, dim3(static_cast<uint32_t>(ctas)), dim3(JOIN_WARPS * 32), 0, a.st, a.b, a.heads, a.chunks,
+                      static_cast<const float*>(a.part), static_cast<const float*>(a.part_ml), static_cast<OUT*>(a.out), a.ldo, a.status);
+}
 template <int DIM>
 cudaError_t launch_join(const AttendCall& a) {
-    const dim3 grid(static_cast<uint32_t>((static_cast<uint64_t>(a.b.rows) * a.heads + JOIN_WARPS - 1) / JOIN_WARPS)), block(JOIN_WARPS * 32);
-    if (a.out_dtype == HF2Q_DT_F32) return launch_pdl(join_kernel<DIM, float>, grid, block, 0, a.st, a.b, a.heads, a.chunks, a.part, a.part_ml, static_cast<float*>(a.out), a.ldo, a.status);
-    if (a.out_dtype == HF2Q_DT_F16) return launch_pdl(join_kernel<DIM, __half>, grid, block, 0, a.st, a.b, a.heads, a.chunks, a.part, a.part_ml, static_cast<__half*>(a.out), a.ldo, a.status);
-    return launch_pdl(join_kernel<DIM, __nv_bfloat16>, grid, block, 0, a.st, a.b, a.heads, a.chunks, a.part, a.part_ml, static_cast<__nv_bfloat16*>(a.out), a.ldo, a.status);
+    return a.out_dtype == HF2Q_DT_F32 ? launch_join_out<DIM, float>(a) : a.out_dtype == HF2Q_DT_F16 ? launch_join_out<DIM, __half>(a) : launch_join_out<DIM, __nv_bfloat16>(a);
 }
 
 // How a call is laid out, from the bounds that the host knows.
@@ -91,10 +129,21 @@ Plan plan_of(const hf2q_pages& c, const hf2q_page_batch& b, uint32_t heads, uint
             const double cost = (seqs == 1 ? std::ceil(tiles * parts / places) * one : std::max(one, all / places + 0.5 * one)) + join;
             if (parts == 1 || cost < best) { best = cost; chunk = size; }
         }
-    } else if (tiles < static_cast<uint64_t>(sms)) {
-        // few tiles: a part for each SM, of no fewer than eight blocks
-        chunk = std::max<uint64_t>(512, (tiles * seen + sms - 1) / sms);
-        chunk = (std::max(chunk, (seen + 255) / 256) + 127) / 128 * 128;
+    } else {
+        // In units of 64 positions of a CTA (1.7 us): it takes 8 of them to begin and end, there is one CTA on an SM, and joining takes 2 and reads and
+        // writes every part (2.5 MB a us).  Tiles of one length: whole rounds.  Of several, from several sequences or from a prompt that is long against
+        // what is before it: what they take together, and half of one part for the end.  (64 rows of 8 heads after 32768 positions: 18 parts, one round,
+        // 87 us; 20 parts 136; 8 parts 133.  640 rows after 8192: 1 part 246, 3 parts 202, 7 parts 231.)
+        const bool even = seqs == 1 && (seen < ceil128 || 4ull * b.max_new <= seen);
+        const double places = sms, held = even || seen < ceil128 ? 1.0 : (b.max_length - b.max_new / 2) / static_cast<double>(std::max(1u, b.max_length));
+        const double bytes = static_cast<double>(b.rows) * heads * c.dim * 8.0;
+        double best = 0.0;
+        for (uint64_t parts = 1; parts <= 256 && (parts == 1 || seen / parts >= 256); ++parts) {
+            const uint64_t size = ((seen + parts - 1) / parts + 127) / 128 * 128, count = (seen + size - 1) / size;
+            const double one = 8.0 + size / 64.0, rounds = tiles * count / places, join = count > 1 ? 2.0 + count * bytes / 4.2e6 : 0.0;
+            const double cost = (even ? std::ceil(rounds) * one : std::max(one, rounds * held * one + 0.5 * one)) + join;
+            if (parts == 1 || cost < best) { best = cost; chunk = size; }
+        }
     }
     p.chunks = static_cast<uint32_t>((seen + chunk - 1) / chunk);
     p.chunk = static_cast<uint32_t>(chunk);

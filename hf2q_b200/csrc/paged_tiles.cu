@@ -165,6 +165,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
     __shared__ uint32_t tmem_slot;
     const uint32_t kvh = blockIdx.x % c.kv_heads, chunk = blockIdx.y, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     uint32_t seq = 0, tok0 = 0;
+    pdl_wait();
     if (blockIdx.x == 0 && chunk == 0)                                    // (a sequence that does not fit may have no tile to say so)
         for (uint32_t s = threadIdx.x; s < b.seqs; s += THREADS)
             if (span_of(b, c.shift, s).bad) atomicOr(status, STATUS_BAD_PAGE);
@@ -237,6 +238,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_trigger();                                                        // (not before the columns are held: a launch behind may take them and then wait for this one)
     const uint32_t tmem = tmem_slot;
     const float scale = fabsf(look.scale);
 
@@ -673,13 +675,13 @@ cudaError_t launch(const AttendCall& a) {
     const auto kern = attend_tiles_kernel<DIM, CODES, Q, OUT>;
     if (const cudaError_t e = ensure_max_dynamic_smem(kern, smem, flag); e != cudaSuccess) return e;
     const uint32_t group = a.heads / a.c.kv_heads, tokens = ROWS / group;
-    const uint64_t tiles = a.b.rows / (2 * tokens) + std::min(a.b.seqs, a.b.rows);      // at most: each sequence's last tile may be a part
+    // at most: each sequence's last tile may be a part
+    const uint64_t per = 2 * tokens, seqs = std::min(a.b.seqs, a.b.rows), tiles = std::min(a.b.rows / per + seqs, seqs * ((a.b.max_new + per - 1) / per));
     if (tiles * a.c.kv_heads > 0x7fffffffull) return cudaErrorInvalidValue;
     const bool wide = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.ldq % (16 / sizeof(Q)) == 0;
     const Shape sh{a.heads, group, tokens, a.ldq, a.ldo, a.chunk >> BP_LOG, a.chunks, wide};
-    kern<<<dim3(static_cast<uint32_t>(tiles) * a.c.kv_heads, a.chunks), THREADS, smem, a.st>>>(a.c, a.b, a.look, sh, static_cast<const Q*>(a.q), static_cast<OUT*>(a.out), a.part, a.part_ml,
-                                                                                              a.status);
-    return cudaGetLastError();
+    return launch_pdl(kern, dim3(static_cast<uint32_t>(tiles) * a.c.kv_heads, a.chunks), dim3(THREADS), smem, a.st, a.c, a.b, a.look, sh, static_cast<const Q*>(a.q),
+                      static_cast<OUT*>(a.out), a.part, a.part_ml, a.status);
 }
 template <int DIM, bool CODES, typename Q>
 cudaError_t launch_out(const AttendCall& a) {
