@@ -131,18 +131,22 @@ Plan plan_of(const hf2q_pages& c, const hf2q_page_batch& b, uint32_t heads, uint
         }
     } else {
         // In units of 64 positions of a CTA (1.7 us): it takes 8 of them to begin and end, there is one CTA on an SM, and joining takes 2 and reads and
-        // writes every part (2.5 MB a us).  Tiles of one length: whole rounds.  Of several, from several sequences or from a prompt that is long against
-        // what is before it: what they take together, and half of one part for the end.  (64 rows of 8 heads after 32768 positions: 18 parts, one round,
-        // 87 us; 20 parts 136; 8 parts 133.  640 rows after 8192: 1 part 246, 3 parts 202, 7 parts 231.)
-        const bool even = seqs == 1 && (seen < ceil128 || 4ull * b.max_new <= seen);
-        const double places = sms, held = even || seen < ceil128 ? 1.0 : (b.max_length - b.max_new / 2) / static_cast<double>(std::max(1u, b.max_length));
+        // writes every part (2.5 MB a us).  Whole rounds, as if all sequences were of the largest length: a few CTAs too many cost a round, some SMs
+        // left over little.  (The last part is the shortest, so that one may follow another on an SM.)  A prompt that is long against what is before
+        // it has tiles of all lengths: what they take together, and half of one part for the end.  (64 rows of 8 heads after 32768 positions: 19 parts
+        // 71 us, 18 75, 20 120, 8 132.  640 rows after 8192: 1 part 246, 3 parts 185, 7 parts 217.  Eight sequences, 5 rows of 4 heads after 3001: 4 parts 23,
+        // 5 parts 33; 22 both where they are of 1500 to 3001.)
+        const bool even = seen < ceil128 || 4ull * b.max_new <= seen;
+        const double places = sms, held = (b.max_length - b.max_new / 2) / static_cast<double>(std::max(1u, b.max_length));
         const double bytes = static_cast<double>(b.rows) * heads * c.dim * 8.0;
         double best = 0.0;
         for (uint64_t parts = 1; parts <= 256 && (parts == 1 || seen / parts >= 256); ++parts) {
-            const uint64_t size = ((seen + parts - 1) / parts + 127) / 128 * 128, count = (seen + size - 1) / size;
-            const double one = 8.0 + size / 64.0, rounds = tiles * count / places, join = count > 1 ? 2.0 + count * bytes / 4.2e6 : 0.0;
-            const double cost = (even ? std::ceil(rounds) * one : std::max(one, rounds * held * one + 0.5 * one)) + join;
-            if (parts == 1 || cost < best) { best = cost; chunk = size; }
+            const uint64_t size = ((seen + parts - 1) / parts + 127) / 128 * 128, count = (seen + size - 1) / size, ctas = tiles * count, full = tiles * (count - 1);
+            const double one = 8.0 + size / 64.0, end = 8.0 + (seen - (count - 1) * size) / 64.0, join = count > 1 ? 2.0 + count * bytes / 4.2e6 : 0.0;
+            double cost = std::ceil(ctas / places) * one;
+            if (full < static_cast<uint64_t>(sms) && ctas > static_cast<uint64_t>(sms) && ctas - sms <= sms - full) cost = std::max(one, 2.0 * end);
+            if (!even) cost = std::max(one, ctas / places * held * one + 0.5 * one);
+            if (parts == 1 || cost + join < best) { best = cost + join; chunk = size; }
         }
     }
     p.chunks = static_cast<uint32_t>((seen + chunk - 1) / chunk);

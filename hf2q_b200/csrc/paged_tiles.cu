@@ -122,7 +122,7 @@ template <typename Q> __device__ __forceinline__ void load8(const Q* p, bool wid
 }
 
 struct Shape {
-    uint32_t heads, group, tokens;           // tokens of a tile
+    uint32_t heads, group, inv_group, tokens;           // inv_group: r * inv_group >> 16 = r / group for r < 128; tokens of a tile
     uint32_t ldq, ldo, chunk_blocks, chunks;
     bool wide_q;
 };
@@ -219,12 +219,13 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
     if (warp == ISSUE_WARP) claim_columns(&tmem_slot);
     // Q: two tiles of 128 rows in 16 bits; a negative scale is taken over by q, so that the largest product is the largest score
     bool clipped = false;
-    for (uint32_t i = threadIdx.x; i < 2 * ROWS * (DIM / 8); i += THREADS) {
-        const uint32_t ch = i % (DIM / 8), r = i / (DIM / 8), tile = r >> 7, rr = r & 127, in_tile = rr / sh.group, tok = tok0 + tile * sh.tokens + in_tile;
+#pragma unroll 2
+    for (uint32_t i = threadIdx.x; i < tiles * ROWS * (DIM / 8); i += THREADS) {
+        const uint32_t ch = i % (DIM / 8), r = i / (DIM / 8), tile = r >> 7, rr = r & 127, in_tile = rr * sh.inv_group >> 16, tok = tok0 + tile * sh.tokens + in_tile;
         uint4 w = make_uint4(0u, 0u, 0u, 0u);
         if (in_tile < sh.tokens && tok < end_tok) {
             float e[8];
-            load8(q + static_cast<size_t>(span.row0 + tok) * sh.ldq + static_cast<size_t>(kvh * sh.group + rr % sh.group) * DIM + 8 * ch, sh.wide_q, e);
+            load8(q + static_cast<size_t>(span.row0 + tok) * sh.ldq + static_cast<size_t>(kvh * sh.group + rr - in_tile * sh.group) * DIM + 8 * ch, sh.wide_q, e);
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
                 if (look.scale < 0.f) e[x] = -e[x];
@@ -292,33 +293,35 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
                     if (!ok) break;
 #pragma unroll
                     for (uint32_t i = 0; i < NP; ++i) store_codes(stages + st * KV_BYTES, RP * i + row0, ch, x[u][i]);
+                    const float2 s = sc[u];
+                    if (j + 2 < nb) {
+                        reach_block(j + 2);
+                        load(j + 2, u);
+                    }
                     float f = scale;
                     if (!keys) {
                         const uint32_t p0 = blocks.at(lo + j) << BP_LOG;
                         const bool all = all_see(look, first, last, p0, BP);
                         float top = 0.f;
-                        if (fabsf(sc[u].x) < CUDART_INF_F && (all || some_see(look, first, last, p0 + 2 * lane))) top = fabsf(sc[u].x);
-                        if (fabsf(sc[u].y) < CUDART_INF_F && (all || some_see(look, first, last, p0 + 2 * lane + 1))) top = fmaxf(top, fabsf(sc[u].y));
+                        if (fabsf(s.x) < CUDART_INF_F && (all || some_see(look, first, last, p0 + 2 * lane))) top = fabsf(s.x);
+                        if (fabsf(s.y) < CUDART_INF_F && (all || some_see(look, first, last, p0 + 2 * lane + 1))) top = fmaxf(top, fabsf(s.y));
                         unit = fmaxf(unit, unit_above(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)))));       // (of numbers >= 0 the order is that of their bits)
                         f = __uint_as_float((258u << 23) - __float_as_uint(unit));          // UNITS / unit, of powers of two
                         if (tid == 0) s_unit[slot] = unit;
                     }
-                    if (lane >> 3 == (warp & 3)) *reinterpret_cast<float2*>(&(keys ? s_ks : s_vs)[slot][2 * lane]) = make_float2(sc[u].x * f, sc[u].y * f);
+                    if (lane >> 3 == (warp & 3)) *reinterpret_cast<float2*>(&(keys ? s_ks : s_vs)[slot][2 * lane]) = make_float2(s.x * f, s.y * f);
                     proxy_fence();
                     __syncwarp();
                     if (lane == 0) {
                         mbar_arrive(&sc_full[slot]);
                         mbar_arrive(&full_bars[st]);
                     }
-                    if (j + 2 < nb) {
-                        reach_block(j + 2);
-                        load(j + 2, u);
-                    }
                 }
             }
         } else {
             const uint32_t to0 = smem_u32(stages) + chunk_at(row0, ch, PANEL);       // (a pass is 8 rows or a multiple: the swizzle of a thread's chunk stays)
             uint32_t met = 0;
+            constexpr int AHEAD = 3;                                      // blocks on their way: the next is asked for when the first was handed over
             auto bring = [&](uint32_t j) {                                // block j, as a group of copies
                 const uint32_t st = j % STAGES, p0 = blocks.at(lo + j) << BP_LOG, to = to0 + st * KV_BYTES;
                 reach_block(j);
@@ -334,17 +337,13 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
                 }
                 copies_close();
             };
-            bring(0);
-            if (nb > 1) bring(1);
+            for (uint32_t j = 0; j < AHEAD; ++j) {
+                if (j < nb) bring(j); else copies_close();
+            }
 #pragma unroll 1
             for (uint32_t j = 0; j < nb && ok; ++j) {
                 const uint32_t st = j % STAGES, p0 = blocks.at(lo + j) << BP_LOG;
-                if (j + 2 < nb) {
-                    bring(j + 2);
-                    if (!ok) break;
-                    copies_wait<2>();
-                } else if (j + 1 < nb) copies_wait<1>();
-                else copies_wait<0>();
+                copies_wait<AHEAD - 1>();
                 if (!keys && !all_see(look, first, last, p0, BP) && first != last) {
                     uint8_t* to = stages + st * KV_BYTES + chunk_at(row0, ch, PANEL);
                     bool odd = false;
@@ -366,6 +365,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
                 proxy_fence();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full_bars[st]);
+                if (j + AHEAD < nb) bring(j + AHEAD); else copies_close();
             }
             copies_wait<0>();
         }
@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
     } else {
         more_registers<SOFTMAX_REGS>();
         const uint32_t tile = warp / 4, row = threadIdx.x & 127, at = tmem + (((warp & 3) * 32u) << 16), at_o = at + COL_O + tile * DIM;
-        const uint32_t in_tile = row / sh.group, tile_tok = tok0 + tile * sh.tokens, tile_end = min(tile_tok + sh.tokens, end_tok), tok = tile_tok + in_tile;
+        const uint32_t in_tile = row * sh.inv_group >> 16, tile_tok = tok0 + tile * sh.tokens, tile_end = min(tile_tok + sh.tokens, end_tok), tok = tile_tok + in_tile;
         const bool live = in_tile < sh.tokens && tok < end_tok, held = live && tok >= lost;
         const uint32_t seen = before + max(min(tok, tile_end - 1), lost);          // (rows that are not there compute on zeros and are not stored)
         const uint32_t t_first = before + max(tile_tok, lost), t_last = before + max(tile_end - 1, lost);
@@ -634,31 +634,54 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
             OUT* dst = out + orow * sh.ldo + head * DIM;
             const size_t at_part = (orow * sh.heads + head) * sh.chunks + chunk;
             const bool wide = reinterpret_cast<uintptr_t>(dst) % 16 == 0;
-            if (sh.chunks > 1 && live) *reinterpret_cast<float2*>(part_ml + 2 * at_part) = make_float2(mx, l);
-            __syncwarp();
+            if (sh.chunks > 1) {
+                // A thread has a row of numbers; parts are written by half-warps, half the columns at a time through what Q has left (a row by each thread
+                // would be 32 lines a store).
+                if (live) *reinterpret_cast<float2*>(part_ml + 2 * at_part) = make_float2(mx, l);
+                const uint32_t rows_live = __ballot_sync(0xffffffffu, live);
+                constexpr uint32_t HALF = DIM / 2, CH = HALF / 4;
+                float4* stage = reinterpret_cast<float4*>(qs + tile * Q_BYTES + (warp & 3) * (Q_BYTES / 4));
 #pragma unroll 1
-            for (uint32_t col = 0; col < DIM; col += 16) {
-                uint32_t o[16];
-                tmem_ld16(at_o + col, o);
-                tmem_wait_ld();
-                if (live && sh.chunks > 1) {
+                for (uint32_t half = 0; rows_live && half < 2; ++half) {
+#pragma unroll 1
+                    for (uint32_t c4 = 0; c4 < CH; c4 += 4) {
+                        uint32_t o[16];
+                        tmem_ld16(at_o + half * HALF + 4 * c4, o);
+                        tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        reinterpret_cast<float4*>(part + at_part * DIM + col)[i] = make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
-                                                                                               __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
-                } else if (live) {
-                    __align__(16) OUT h[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) h[i] = out_value<OUT>(l == 0.f ? 0.f : __uint_as_float(o[i]) * inv, clipped);
-                    if (wide) {
-#pragma unroll
-                        for (int i = 0; i < static_cast<int>(sizeof(OUT)); ++i) reinterpret_cast<uint4*>(dst + col)[i] = reinterpret_cast<const uint4*>(h)[i];
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) dst[col + i] = h[i];
+                        for (uint32_t i = 0; i < 4; ++i)
+                            stage[lane * CH + ((c4 + i) ^ (lane % CH))] = make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
+                                                                                     __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
                     }
+                    __syncwarp();
+#pragma unroll 4
+                    for (uint32_t r0 = 0; r0 < 32; r0 += 32 / CH) {
+                        const uint32_t r = r0 + lane / CH, ch = lane % CH;
+                        float* to = part + __shfl_sync(0xffffffffu, static_cast<unsigned long long>(at_part), r) * DIM + half * HALF + 4 * ch;
+                        if (rows_live >> r & 1) *reinterpret_cast<float4*>(to) = stage[r * CH + (ch ^ (r % CH))];
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();                                             // the next load from tensor memory is the whole warp's
+            } else {
+#pragma unroll 1
+                for (uint32_t col = 0; col < DIM; col += 16) {
+                    uint32_t o[16];
+                    tmem_ld16(at_o + col, o);
+                    tmem_wait_ld();
+                    if (live) {
+                        __align__(16) OUT h[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) h[i] = out_value<OUT>(l == 0.f ? 0.f : __uint_as_float(o[i]) * inv, clipped);
+                        if (wide) {
+#pragma unroll
+                            for (int i = 0; i < static_cast<int>(sizeof(OUT)); ++i) reinterpret_cast<uint4*>(dst + col)[i] = reinterpret_cast<const uint4*>(h)[i];
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) dst[col + i] = h[i];
+                        }
+                    }
+                    __syncwarp();                                         // the next load from tensor memory is the whole warp's
+                }
             }
         }
         tc_fence_before();
@@ -679,7 +702,7 @@ cudaError_t launch(const AttendCall& a) {
     const uint64_t per = 2 * tokens, seqs = std::min(a.b.seqs, a.b.rows), tiles = std::min(a.b.rows / per + seqs, seqs * ((a.b.max_new + per - 1) / per));
     if (tiles * a.c.kv_heads > 0x7fffffffull) return cudaErrorInvalidValue;
     const bool wide = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.ldq % (16 / sizeof(Q)) == 0;
-    const Shape sh{a.heads, group, tokens, a.ldq, a.ldo, a.chunk >> BP_LOG, a.chunks, wide};
+    const Shape sh{a.heads, group, 65536 / group + 1, tokens, a.ldq, a.ldo, a.chunk >> BP_LOG, a.chunks, wide};
     return launch_pdl(kern, dim3(static_cast<uint32_t>(tiles) * a.c.kv_heads, a.chunks), dim3(THREADS), smem, a.st, a.c, a.b, a.look, sh, static_cast<const Q*>(a.q),
                       static_cast<OUT*>(a.out), a.part, a.part_ml, a.status);
 }
