@@ -135,9 +135,9 @@ class PagedCache:
                     _refuse(f"{name} must be [layers, pages, kv_heads, page]")
         self.ctx, self.k, self.v, self.k_scale, self.v_scale = ctx, k, v, k_scale, v_scale
         self.layers, self.pages, self.kv_heads, self.page, self.dim = k.shape
-        at = lambda t, layer: None if t is None else t[layer].data_ptr()
-        self.structs = [_Pages(at(k, i), at(v, i), at(k_scale, i), at(v_scale, i), self.pages, self.page, self.kv_heads, self.dim, DT_I8 if codes else DT_BF16)
-                         for i in range(self.layers)]
+        step = lambda t: 0 if t is None else t.stride(0) * t.element_size()
+        first = [(0 if t is None else t.data_ptr(), step(t)) for t in (k, v, k_scale, v_scale)]
+        self.structs = [_Pages(*(p + i * n or None for p, n in first), self.pages, self.page, self.kv_heads, self.dim, DT_I8 if codes else DT_BF16) for i in range(self.layers)]
         self._refs, self._scale = [C.byref(s) for s in self.structs], self.dim ** -0.5
         self._append, self._attend = ctx._lib.hf2q_cuda_pages_append, ctx._lib.hf2q_cuda_pages_attend
 
