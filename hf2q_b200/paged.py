@@ -98,8 +98,8 @@ class PagedBatch:
             _refuse("a batch of n sequences has n + 1 starts, n lengths and n rows of page numbers")
         if table.stride(1) != 1 and table.shape[1] > 1 or seqs > 1 and table.stride(0) < table.shape[1]:
             _refuse("the page numbers of a sequence lie side by side")
-        if not 0 <= max_new <= rows or not max_new <= max_length:
-            _refuse("max_new is at most rows and at most max_length")
+        if not 0 <= max_new <= rows <= 1 << 28 or not max_new <= max_length <= 1 << 30:
+            _refuse("max_new is at most rows (2^28) and at most max_length (2^30)")
         self.ctx, self._keep = ctx, (start, length, table)
         self.rows, self.max_new, self.max_length = int(rows), int(max_new), int(max_length)
         self.struct = _PageBatch(start.data_ptr(), length.data_ptr(), table.data_ptr(), seqs, self.rows, table.stride(0) if seqs > 1 else table.shape[1],
@@ -177,8 +177,8 @@ class PagedCache:
         ctx, rows, width = self.ctx, batch.rows, heads * self.dim
         self._check(layer, batch)
         ldq, ldo = _rows(q, "q", _IN, rows, width, ctx), _rows(out, "out", _OUT, rows, width, ctx)
-        if window < 0 or sinks < 0:
-            _refuse("window and sinks are not negative")
+        if not (0 <= window < 1 << 32 and 0 <= sinks < 1 << 32):
+            _refuse("window and sinks are not negative, and below 2^32")
         scratch = batch.scratch(self.structs[layer], heads, window, sinks)
         rc = self._attend(ctx._h, ctx._stream(), self._refs[layer], batch.ref, q.data_ptr(), _TORCH_DT[q.dtype], ldq, heads, self._scale if scale is None else scale, window, sinks,
                           out.data_ptr(), _TORCH_DT[out.dtype], ldo, scratch.data_ptr(), scratch.numel())

@@ -14,19 +14,19 @@ def _without_pages(pages) -> None:
         raise ops.Hf2qError(_lib.ERR_INVALID_ARGUMENT, "this design keeps its sequences in rings and states, not in pages")
 
 
-def _fomatar(ctx, path, dtype, max_seq, n_slots, prefill_chunk, pages):
+def _fomatar(ctx, path, dtype, max_seq, n_slots, prefill_chunk, pages=None):
     _without_pages(pages)
     from .fomatar import FomatarDecoder
     return FomatarDecoder.from_directory(ctx, path, dtype=dtype, max_seq=max_seq, n_slots=n_slots, prefill_chunk=prefill_chunk)
 
 
-def _runopel(ctx, path, dtype, max_seq, n_slots, prefill_chunk, pages):
+def _runopel(ctx, path, dtype, max_seq, n_slots, prefill_chunk, pages=None):
     _without_pages(pages)
     from .runopel import RunopelDecoder
     return RunopelDecoder.from_directory(ctx, path, dtype=dtype, max_seq=max_seq, n_slots=n_slots, prefill_chunk=prefill_chunk)
 
 
-def _llama(ctx, path, dtype, max_seq, n_slots, prefill_chunk, pages):
+def _llama(ctx, path, dtype, max_seq, n_slots, prefill_chunk, pages=None):
     from .decoder import LlamaDecoder
     if dtype != torch.bfloat16:
         raise ops.Hf2qError(_lib.ERR_INVALID_ARGUMENT, "the quantized decoder has no 32-bit mode")
@@ -55,4 +55,4 @@ def load_model(ctx: ops.GpuContext, path, dtype=torch.bfloat16, max_seq: int = 3
     arch = architecture_of(path)
     if arch not in ARCHITECTURES:
         raise ops.Hf2qError(_lib.ERR_INVALID_ARGUMENT, f"architecture '{arch}' is not registered (have: {', '.join(sorted(ARCHITECTURES))})")
-    return ARCHITECTURES[arch](ctx, path, dtype, max_seq, n_slots, prefill_chunk, pages)
+    return ARCHITECTURES[arch](ctx, path, dtype, max_seq, n_slots, prefill_chunk, *(() if pages is None else (pages,)))

@@ -134,7 +134,8 @@ def test_the_classes_refuse_too(gpu_ctx):
         lambda: cache.copy_rows(torch.zeros(2, device="cuda"), torch.zeros(2, device="cuda")),
         lambda: paged.PagedCache(gpu_ctx, cache.k, cache.v), lambda: paged.PagedCache(gpu_ctx, cache.k, cache.v[:, :1], cache.k_scale, cache.v_scale),
         lambda: paged.PagedCache(gpu_ctx, cache.k, cache.v, cache.k_scale, cache.v_scale[..., :8]), lambda: paged.PagedCache(gpu_ctx, cache.k[0], cache.v[0], cache.k_scale[0], cache.v_scale[0]),
-        lambda: t.pages.batch(gpu_ctx, max_new=9, rows=3), lambda: t.pages.batch(gpu_ctx, max_length=2),
+        lambda: t.pages.batch(gpu_ctx, max_new=9, rows=3), lambda: t.pages.batch(gpu_ctx, max_length=2), lambda: t.pages.batch(gpu_ctx, max_length=1 << 32),
+        lambda: t.pages.batch(gpu_ctx, rows=(1 << 32) + 3), lambda: cache.attend(0, batch_, t.q, 4, t.out, window=1 << 32), lambda: cache.attend(0, batch_, t.q, 4, t.out, sinks=1 << 32),
     ]
     for i, call in enumerate(bad):
         with pytest.raises(Hf2qError):
