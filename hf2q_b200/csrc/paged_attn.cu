@@ -118,16 +118,19 @@ Plan plan_of(const hf2q_pages& c, const hf2q_page_batch& b, uint32_t heads, uint
     const uint64_t tiles = static_cast<uint64_t>(c.kv_heads) * seqs * ((units + rows - 1) / rows);
     uint64_t chunk = seen;
     if (p.step) {
-        // A CTA takes about 4 us to begin and end and 1 us for 64 positions, two CTAs run on an SM, and joining parts takes 3 us.  One sequence: whole
-        // rounds of equal parts.  Several, of several lengths: what they hold together, six tenths of the most (all of it in a window), shared evenly,
-        // and half of one part for the end.  (Of 24 sequences with a window of 1024 in 64 elements: parts of 256 positions 26 us, whole 15 us.)
-        const double places = 2.0 * sms, held = seqs == 1 || seen < ceil128 ? 1.0 : 0.6;
+        // A CTA takes about 4 us to begin and end; 64 positions take 1 us where two CTAs share an SM (half of it with heads of 64), 0.7 where one has it, and
+        // 0.8 of that while the SMs are not full; joining parts takes 3 us.  One sequence: whole rounds of equal parts.  Several, of several lengths: one round as long as there is one;
+        // else what they hold together, 0.65 of the most (all of it in a window), shared evenly, and half of one part for the end.  (Codes, 4 sequences of
+        // up to 30000: 10 parts 47 us, 17 parts 56, 4 parts 89.  32 sequences of up to 8191: 1 part 97, 4 parts 79, 10 parts 88.  16 sequences of up to 2000 in
+        // bf16: 1 part 25, 2 parts 31.  24 sequences with a window of 1024 in 64 elements: whole 12, parts of 512 18.)
+        const uint32_t on_sm = step_ctas(c.dim, c.dtype == HF2Q_DT_I8, units > 8);
+        const double places = static_cast<double>(sms) * on_sm, block = c.dim == 64 ? 0.5 : on_sm > 1 ? 1.0 : 0.7, held = seqs == 1 || seen < ceil128 ? 1.0 : 0.65;
         double best = 0.0;
         for (uint64_t parts = 1; parts <= 256 && (parts == 1 || seen / parts >= 128); ++parts) {
             const uint64_t size = ((seen + parts - 1) / parts + 127) / 128 * 128;
-            const double one = 4.0 + size / 64.0, all = tiles * held * (4.0 * parts + seen / 64.0), join = parts > 1 ? 3.0 : 0.0;
-            const double cost = (seqs == 1 ? std::ceil(tiles * parts / places) * one : std::max(one, all / places + 0.5 * one)) + join;
-            if (parts == 1 || cost < best) { best = cost; chunk = size; }
+            const double one = 4.0 + block * size / 64.0, all = tiles * held * (4.0 * parts + block * seen / 64.0), join = parts > 1 ? 3.0 : 0.0;
+            const double cost = seqs == 1 ? std::ceil(tiles * parts / places) * one : tiles * parts <= places ? 4.0 + 0.8 * block * size / 64.0 : std::max(one, all / places + 0.5 * one);
+            if (parts == 1 || cost + join < best) { best = cost + join; chunk = size; }
         }
     } else {
         // In units of 64 positions of a CTA (1.7 us): it takes 8 of them to begin and end, there is one CTA on an SM, and joining takes 2 and reads and

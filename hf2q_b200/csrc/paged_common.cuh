@@ -101,6 +101,9 @@ cudaError_t launch_attend_tiles(const AttendCall& a, uint32_t dim, bool codes); 
 // what the sums of a part count for beside others: a part that saw nothing has none (its sum is 0), one of NaN scores alone has no maximum
 __device__ __forceinline__ float part_factor(float m, float l, float m_all) { return l == 0.f ? 0.f : m == -INFINITY ? 1.0f : exp2f(m - m_all); }
 
+// CTAs of the few-rows kernel that share an SM (tall: tiles of 16 rows)
+constexpr uint32_t step_ctas(uint32_t dim, bool codes, bool tall) { return dim == 64 || (codes && !tall) ? 2 : 1; }
+
 template <typename OUT> __device__ __forceinline__ OUT out_value(float v, bool& clipped);
 template <> __device__ __forceinline__ float out_value<float>(float v, bool&) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 out_value<__nv_bfloat16>(float v, bool&) { return __float2bfloat16_rn(v); }

@@ -70,7 +70,7 @@ constexpr uint32_t step_smem() { return WARPS * (TALL ? 16 : 8) * (DIM + 4) * 4;
 
 // TALL: tiles of 16 rows, else of 8.  The tile's rows are u = token * group + head of the sequence's new tokens and the KV head's query heads.
 template <int DIM, bool CODES, bool TALL, typename Q, typename OUT>
-__global__ void __launch_bounds__(WARPS * 32, DIM == 64 || (CODES && !TALL) ? 2 : 1)
+__global__ void __launch_bounds__(WARPS * 32, step_ctas(DIM, CODES, TALL))
 attend_step_kernel(Pool c, Batch b, Look look, uint32_t heads, uint32_t group, const Q* q, uint32_t ldq, bool wide_q, OUT* out, uint32_t ldo, uint32_t chunk_steps, uint32_t chunks,
                    float* part, float* part_ml, uint32_t* status) {
     constexpr int R = TALL ? 16 : 8, KS = DIM / 16;                       // rows, contraction steps of a score
