@@ -44,3 +44,52 @@ def test_parts_give_the_same_sums_every_time(gpu_ctx):
             cache.attend(0, batch, q, c.heads, g)
         gpu_ctx.check_status()
         assert all(torch.equal(g, got[0]) for g in got) and not bool(got[0].isnan().any())
+
+
+def test_calls_on_two_streams_at_once(gpu_ctx):
+    """Each with a batch, and so a scratch, of its own; eager and replayed."""
+    sets = []
+    for seed, lengths in enumerate(([(200, 1500), (90, 300)], [(1, 6000), (1, 700)], [(130, 0)], [(40, 2600)])):
+        c = Pages(lengths, 2, 4, 128, 32, torch.int8 if seed % 2 else torch.bfloat16, seed=seed)
+        sets.append((c, c.cache(gpu_ctx), c.q.cuda()))
+    run = lambda s, batch, out: s[1].attend(0, batch, s[2], s[0].heads, out)
+    new = lambda s: torch.empty((s[0].rows, s[0].heads * 128), device="cuda")
+    want = []
+    for s in sets:
+        want.append(new(s))
+        run(s, s[0].batch(gpu_ctx), want[-1])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    batches = [[s[0].batch(gpu_ctx) for s in sets] for _ in streams]
+    outs = [[[new(s) for s in sets] for _ in range(6)] for _ in streams]
+    torch.cuda.synchronize()
+    graphs = []
+    for k, st in enumerate(streams):
+        with torch.cuda.stream(st):
+            for s, b, o in zip(sets, batches[k], outs[k][0]):                       # (makes the scratch)
+                run(s, b, o)
+    torch.cuda.synchronize()
+    for k, st in enumerate(streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            for out in outs[k][3:]:
+                for i in range(len(sets)):
+                    i = i if k == 0 else len(sets) - 1 - i
+                    run(sets[i], batches[k][i], out[i])
+        graphs.append(g)
+    torch.cuda.synchronize()
+    for out in (o for k in outs for o in k):
+        for o in out:
+            o.zero_()
+    torch.cuda.synchronize()
+    for r in range(3):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                for i in range(len(sets)):
+                    i = i if k == 0 else len(sets) - 1 - i
+                    run(sets[i], batches[k][i], outs[k][r][i])
+    for k, st in enumerate(streams):
+        with torch.cuda.stream(st):
+            graphs[k].replay()
+    torch.cuda.synchronize()
+    gpu_ctx.check_status()
+    assert all(torch.equal(o, w) for k in outs for out in k for o, w in zip(out, want))

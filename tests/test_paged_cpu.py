@@ -235,3 +235,12 @@ def test_frequencies():
     # 1257 positions: 2 turns at 0.01, a third of the way between low and high
     g = paged.rope_frequencies(8, 10000.0, bands={"factor": 8.0, "low": 1.0, "high": 4.0, "trained": 400 * 3.141592653589793})
     torch.testing.assert_close(g[2], torch.tensor(0.01 * (1 / 3 + 2 / 3 / 8)), rtol=2 ** -23, atol=0)
+
+
+def test_the_tile_kernel_lets_the_next_launch_start_when_its_columns_are_held():
+    """The next launch may take tensor memory and then wait for this one, whose allocation waits without a limit."""
+    text = (CSRC / "paged_tiles.cu").read_text()
+    body = text[text.index("attend_tiles_kernel("):text.index("cudaError_t launch(")]
+    assert body.count("pdl_trigger()") == 1 and body.count("pdl_wait()") == 1 and body.count("claim_columns(") == 1
+    claim = body.index("claim_columns(")
+    assert body.index("pdl_wait()") < claim < body.index("__syncthreads()", claim) < body.index("pdl_trigger()")
