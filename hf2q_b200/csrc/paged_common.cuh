@@ -101,6 +101,16 @@ cudaError_t launch_attend_tiles(const AttendCall& a, uint32_t dim, bool codes); 
 // what the sums of a part count for beside others: a part that saw nothing has none (its sum is 0), one of NaN scores alone has no maximum
 __device__ __forceinline__ float part_factor(float m, float l, float m_all) { return l == 0.f ? 0.f : m == -INFINITY ? 1.0f : exp2f(m - m_all); }
 
+// How many units of 2^log positions a part has.  A call is laid out for max_length; where up to 32 sequences are all much shorter now, their
+// parts are as much shorter, down to `least`, so that as many CTAs work.  (Whole warps come here.  Either number of units covers all: there
+// are `parts` times as many as the longest sequence has.)
+__device__ __forceinline__ uint32_t part_units(const Batch& b, uint32_t log, uint32_t planned, uint32_t parts, uint32_t least) {
+    if (parts <= 1 || b.seqs > 32) return planned;
+    const uint32_t lane = threadIdx.x & 31, longest = __reduce_max_sync(0xffffffffu, lane < b.seqs ? min(b.length[lane], b.max_length) : 0u);
+    if (4ull * longest > 3ull * b.max_length) return planned;
+    return min(planned, max(least, ((longest + (1u << log) - 1 >> log) + parts - 1) / parts));
+}
+
 // CTAs of the few-rows kernel that share an SM (tall: tiles of 16 rows)
 constexpr uint32_t step_ctas(uint32_t dim, bool codes, bool tall) { return dim == 64 || (codes && !tall) ? 2 : 1; }
 

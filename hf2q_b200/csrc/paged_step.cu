@@ -86,6 +86,7 @@ attend_step_kernel(Pool c, Batch b, Look look, uint32_t heads, uint32_t group, c
     const uint32_t s = blockIdx.z, kvh = blockIdx.x % c.kv_heads, tile = blockIdx.x / c.kv_heads, chunk = blockIdx.y;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, t = lane & 3;
     const Span span = span_of(b, c.shift, s);
+    const uint32_t part_steps = part_units(b, STEP_LOG, chunk_steps, chunks, 8);
     if (span.bad && threadIdx.x == 0 && blockIdx.x == 0 && chunk == 0) atomicOr(status, STATUS_BAD_PAGE);
     const uint32_t u0 = tile * R, units = span.rows * group;
     if (u0 >= units) return;
@@ -95,8 +96,8 @@ attend_step_kernel(Pool c, Batch b, Look look, uint32_t heads, uint32_t group, c
     const bool any = tok1 >= lost;
     const uint32_t first = any ? before + max(tok0, lost) : 0, last = any ? before + tok1 : 0;
     const Blocks blocks = blocks_of(look, first, last, STEP_LOG);
-    const uint32_t lo = static_cast<uint32_t>(min(static_cast<uint64_t>(chunk) * chunk_steps, static_cast<uint64_t>(blocks.count)));
-    const uint32_t hi = any ? min(lo + chunk_steps, blocks.count) : lo;
+    const uint32_t lo = static_cast<uint32_t>(min(static_cast<uint64_t>(chunk) * part_steps, static_cast<uint64_t>(blocks.count)));
+    const uint32_t hi = any ? min(lo + part_steps, blocks.count) : lo;
     if (chunks > 1 && lo >= hi) {                                         // nothing for this part: its sums count for nothing
         for (uint32_t u = u0 + threadIdx.x; u < min(u0 + R, units); u += WARPS * 32)
             *reinterpret_cast<float2*>(part_ml + 2 * (((static_cast<size_t>(span.row0) + u / group) * heads + kvh * group + u % group) * chunks + chunk)) = make_float2(-CUDART_INF_F, 0.f);

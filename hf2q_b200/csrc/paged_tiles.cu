@@ -185,8 +185,9 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
     const bool any = end_tok > lost;
     const uint32_t first = any ? before + max(tok0, lost) : 0, last = any ? before + end_tok - 1 : 0;
     const Blocks blocks = blocks_of(look, first, last, BP_LOG);
-    const uint32_t lo = static_cast<uint32_t>(min(static_cast<uint64_t>(chunk) * sh.chunk_blocks, static_cast<uint64_t>(blocks.count)));
-    const uint32_t nb = any ? min(sh.chunk_blocks, blocks.count - lo) : 0;
+    const uint32_t part_blocks = part_units(b, BP_LOG, sh.chunk_blocks, sh.chunks, 4);
+    const uint32_t lo = static_cast<uint32_t>(min(static_cast<uint64_t>(chunk) * part_blocks, static_cast<uint64_t>(blocks.count)));
+    const uint32_t nb = any ? min(part_blocks, blocks.count - lo) : 0;
     if (nb == 0) {
         // nothing to see here: a part that counts for nothing, or zeros
         const uint32_t units = (end_tok - tok0) * sh.group;

@@ -34,6 +34,29 @@ def test_parts_join_to_the_whole(gpu_ctx, case, dtype, out):
     assert bool((got[:, c.heads * dim:] == 5).all())
 
 
+@pytest.mark.parametrize("case", range(len(CASES)))
+@pytest.mark.parametrize("longer", [1.3, 1.4, 4, 50])
+@pytest.mark.parametrize("window", [0, 500])
+def test_calls_laid_out_for_longer_sequences(gpu_ctx, case, longer, window):
+    """Where all sequences are much shorter than the call allows, the parts are too."""
+    lengths, kv, group, dim, _, _ = CASES[case]
+    c = Pages(lengths, kv, group, dim, 64, torch.int8, seed=case, ld_extra=3)
+    got = torch.empty((c.rows, c.heads * dim), device="cuda")
+    c.cache(gpu_ctx).attend(0, c.batch(gpu_ctx, max_length=int(longer * int(c.length.max()))), c.q.cuda(), c.heads, got, window=window, sinks=5)
+    gpu_ctx.check_status()
+    want, tol = attention(c, c.q, torch.float32, torch.float32, window=window, sinks=5)
+    close(got, want, tol)
+
+
+def test_more_sequences_than_a_warp_has_lanes(gpu_ctx):
+    c = Pages([(1, 60 * i) for i in range(40)], 1, 4, 64, 32, torch.int8, seed=1)
+    got = torch.empty((c.rows, c.heads * 64), device="cuda")
+    c.cache(gpu_ctx).attend(0, c.batch(gpu_ctx, max_length=20000), c.q.cuda(), c.heads, got)
+    gpu_ctx.check_status()
+    want, tol = attention(c, c.q, torch.float32, torch.float32)
+    close(got, want, tol)
+
+
 def test_parts_give_the_same_sums_every_time(gpu_ctx):
     for lengths in ([(1, 9000), (1, 2500)], [(70, 9100)]):
         c = Pages(lengths, 2, 4, 128, 16, torch.int8, seed=3)
