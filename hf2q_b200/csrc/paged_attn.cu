@@ -97,10 +97,12 @@ cudaError_t launch_join(const AttendCall& a) {
 }
 
 // How a call is laid out, from the bounds that the host knows.
-// Rows of a sequence (tokens times heads of a group) that the step kernel takes: one tile of 16; and up to four over short contexts, where the
-// other kernel's start is what takes long (us, step / tiles: 32 rows of 8000 positions 30.2 / 27.6, 64 rows 36.2 / 27.7; 48 rows of 300 positions
-// 14.3 / 17.2, 64 rows of 60 10.3 / 13.2).
-constexpr uint64_t STEP_UNITS = 16, STEP_SHORT_UNITS = 64, STEP_SHORT = 1024;
+// Rows of a sequence (tokens times heads of a group) that the step kernel takes: one tile of 16, with codes two, whatever the context; and up to four as
+// long as all its tiles together go through few positions, since the other kernel takes longer to begin and end but its tiles of 128 rows read
+// them once (us, step / tiles, 8 KV heads.  Codes: 32 rows of 8000 positions 18.1 / 24.8, of 16 sequences of 3000 80 / 85; 64 rows of 300 10.3 / 16.1, of 8000
+// 23.8 / 25.8, of 32768 68 / 54, of 16 sequences of 3000 116 / 89.  bf16: 64 rows of 1000 12.2 / 15.2, 32 rows of 32768 49 / 41; 4 KV heads, 35 rows of 8 sequences
+// of up to 3001 30 / 22).
+constexpr uint64_t STEP_UNITS = 16, STEP_UNITS_CODES = 32, STEP_UNITS_MOST = 64, STEP_WORK = 1 << 17, STEP_WORK_CODES = 1 << 18;
 struct Plan {
     bool step;
     uint32_t chunk, chunks;
@@ -109,7 +111,10 @@ struct Plan {
 Plan plan_of(const hf2q_pages& c, const hf2q_page_batch& b, uint32_t heads, uint32_t window, uint32_t sinks, int sms) {
     Plan p{};
     const uint64_t group = heads / c.kv_heads, units = b.max_new * group;
-    p.step = units <= STEP_UNITS || (units <= STEP_SHORT_UNITS && b.max_length <= STEP_SHORT);
+    const bool codes = c.dtype == HF2Q_DT_I8;
+    const uint64_t most = window ? std::min<uint64_t>(b.max_length, static_cast<uint64_t>(window) + b.max_new + sinks) : b.max_length;
+    const uint64_t work = most * c.kv_heads * std::min(b.seqs, b.rows) * ((units + 15) / 16);
+    p.step = units <= (codes ? STEP_UNITS_CODES : STEP_UNITS) || (units <= STEP_UNITS_MOST && work <= (codes ? STEP_WORK_CODES : STEP_WORK));
     const uint64_t rows = units <= 8 ? 8 : p.step ? 16 : 2 * (128 / group) * group;
     // most positions that a tile goes through, and tiles as if every sequence that can have rows had the most
     const uint64_t ceil128 = (b.max_length + 127ull) / 128 * 128, seqs = std::min(b.seqs, b.rows);
