@@ -124,6 +124,7 @@ class PagedLlamaDecoder(LlamaDecoder):
             return torch.empty(0, dtype=torch.int32, device=self.dev) if collect else None
         with self._ordered():
             self._reserve(n)
+            self.pos.fill_(self.pages.length_of(self._slot))         # (the pool may have compacted the sequence)
             out = super().generate(n, use_graph, collect)
             self.pages.advance(self._slot, n)
         return out

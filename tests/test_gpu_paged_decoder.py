@@ -110,6 +110,29 @@ def test_packed_pages_keep_the_sequences(gpu_ctx, weights, dec):
     dec.ctx.check_status()
 
 
+def test_compacted_sequences_go_on_where_they_end(gpu_ctx, weights, dec):
+    """Back to a prefix of 70 tokens: what follows is what follows that prefix."""
+    ids, more = tokens(16, 70), tokens(17, 3)
+    d = PagedLlamaDecoder(gpu_ctx, CFG, weights[0], prefill_chunk=32, n_slots=1, pages=8)
+    s = d.open_slot()
+    d.extend(s, ids, [])
+    want_first = d.tok.clone()
+    want = d.generate(4).tolist()
+    x = dec.open_slot()
+    dec.extend(x, ids, [])
+    assert torch.equal(dec.tok, want_first)
+    y = dec.fork(x)
+    dec.extend(y, more, [])
+    dec.generate(2)
+    dec.pages.compact(y, range(70))
+    dec.tok.copy_(want_first)
+    assert dec.generate(4).tolist() == want
+    assert int(dec.pos[0]) == 74 == dec.pages.length_of(y)
+    dec.bind(x)
+    assert dec.generate(4).tolist() == want
+    dec.ctx.check_status()
+
+
 def test_calls_on_several_streams_follow_one_another(gpu_ctx, weights, dec):
     ids = tokens(9, 90)
     want = alone(gpu_ctx, weights, [ids[:60], ids[60:]], 5)
