@@ -602,6 +602,10 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
             tmem_wait_st();
             if constexpr (!CODES) {
                 if (odd) {
+                    // What blocks before gave has to be there before it is read and written back (S(j), which this warp has seen, says nothing about it).
+                    if (j) ok = __all_sync(0xffffffffu, ok && wait(&o_done[tile], (j - 1) & 1, status));
+                    if (!ok) break;
+                    tc_fence_after();
 #pragma unroll 1
                     for (uint32_t p16 = 0; p16 < BP / 16; ++p16) {
                         uint32_t w[16];
