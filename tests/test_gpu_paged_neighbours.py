@@ -20,7 +20,8 @@ AT = {0: 3, 1: 17}                                                    # the elem
 def test_finite_elements_are_right_beside_bad_ones(gpu_ctx, values, new, before, group, dim, window, sinks):
     c, clean = (Pages([(new, before), (2, 9)], 2, group, dim, 16, BF, new + before) for _ in "ab")
     total = before + new
-    bad = torch.arange(max(0, before - window if window else before) + 5, total, 13)
+    first = max(0, before - window) + 5 if window else before + 5
+    bad = torch.arange(first, first + 60 if window else total, 13)                                      # (a window: the last rows have left them behind)
     for n, p in enumerate(bad.tolist()):
         for head, d in AT.items():
             c.v[0, int(c.table[0, p // 16]), head, p % 16, d] = values[n % len(values)]
