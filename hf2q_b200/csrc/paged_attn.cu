@@ -117,7 +117,7 @@ Plan plan_of(const hf2q_pages& c, const hf2q_page_batch& b, uint32_t heads, uint
     p.step = units <= (codes ? STEP_UNITS_CODES : STEP_UNITS) || (units <= STEP_UNITS_MOST && work <= (codes ? STEP_WORK_CODES : STEP_WORK));
     const uint64_t rows = units <= 8 ? 8 : p.step ? 16 : 2 * (128 / group) * group;
     // most positions that a tile goes through, and tiles as if every sequence that can have rows had the most
-    const uint64_t ceil128 = (b.max_length + 127ull) / 128 * 128, seqs = std::min(b.seqs, b.rows);
+    const uint64_t ceil128 = (std::max(1u, b.max_length) + 127ull) / 128 * 128, seqs = std::min(b.seqs, b.rows);
     uint64_t seen = ceil128;
     if (window) seen = std::min<uint64_t>(seen, (static_cast<uint64_t>(window) + b.max_new + sinks + (p.step ? 32 : 256) + 127) / 128 * 128);
     const uint64_t tiles = static_cast<uint64_t>(c.kv_heads) * seqs * ((units + rows - 1) / rows);
@@ -159,7 +159,7 @@ Plan plan_of(const hf2q_pages& c, const hf2q_page_batch& b, uint32_t heads, uint
     }
     p.chunks = static_cast<uint32_t>((seen + chunk - 1) / chunk);
     p.chunk = static_cast<uint32_t>(chunk);
-    p.scratch = p.chunks > 1 ? (static_cast<uint64_t>(b.rows) * heads * p.chunks * (c.dim + 2) * 4 + 255) / 256 * 256 : 256;
+    p.scratch = p.chunks > 1 && b.rows ? (static_cast<uint64_t>(b.rows) * heads * p.chunks * (c.dim + 2) * 4 + 255) / 256 * 256 : 256;
     return p;
 }
 
