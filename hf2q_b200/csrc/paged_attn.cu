@@ -192,13 +192,14 @@ HF2Q_API int32_t hf2q_cuda_pages_attend(hf2q_ctx* ctx, void* stream, const hf2q_
     if (const char* e = pages_error(c)) return refuse(ctx, who, e);
     if (const char* e = batch_error(b)) return refuse(ctx, who, e);
     if (const char* e = heads_error(c, heads)) return refuse(ctx, who, e);
-    if (!q || !out) return refuse(ctx, who, "null pointer");
+    const bool none = b->rows == 0 || b->max_new == 0;                    // (arrays without elements have no address)
+    if (!none && (!q || !out)) return refuse(ctx, who, "null pointer");
     if (q_dtype != HF2Q_DT_F32 && q_dtype != HF2Q_DT_BF16) return refuse(ctx, who, "q is F32 or BF16");
     if (out_dtype != HF2Q_DT_F32 && out_dtype != HF2Q_DT_BF16 && out_dtype != HF2Q_DT_F16) return refuse(ctx, who, "out is F32, BF16 or F16");
     const uint64_t width = static_cast<uint64_t>(heads) * c->dim;
     if (ldq < width || ldo < width) return refuse(ctx, who, "rows overlap (ldq or ldo is too small)");
     if (reinterpret_cast<uintptr_t>(q) % (q_dtype == HF2Q_DT_F32 ? 4 : 2) || reinterpret_cast<uintptr_t>(out) % (out_dtype == HF2Q_DT_F32 ? 4 : 2)) return refuse(ctx, who, "rows start between two elements");
-    if (b->rows == 0 || b->max_new == 0) return HF2Q_OK;
+    if (none) return HF2Q_OK;
     const Plan p = plan_of(*c, *b, heads, window, sinks, ctx_sm_count(ctx));
     if (!scratch || scratch_bytes < p.scratch) return ctx_fail(ctx, HF2Q_ERR_WORKSPACE, "pages_attend: scratch missing or too small (ask hf2q_cuda_pages_attend_scratch_bytes)");
     if (reinterpret_cast<uintptr_t>(scratch) % 256) return refuse(ctx, who, "scratch is 256-byte aligned");

@@ -304,7 +304,7 @@ HF2Q_API int32_t hf2q_cuda_pages_append(hf2q_ctx* ctx, void* stream, const hf2q_
     const char* who = "pages_append";
     if (const char* e = pages_error(c)) return refuse(ctx, who, e);
     if (const char* e = batch_error(b)) return refuse(ctx, who, e);
-    if (!x || (heads && !q_out)) return refuse(ctx, who, "null pointer");
+    if (b->rows && (!x || (heads && !q_out))) return refuse(ctx, who, "null pointer");       // (arrays without elements have no address)
     if ((x_dtype != HF2Q_DT_F32 && x_dtype != HF2Q_DT_BF16) || (heads && q_dtype != HF2Q_DT_F32 && q_dtype != HF2Q_DT_BF16)) return refuse(ctx, who, "rows are F32 or BF16");
     if (heads > 65535) return refuse(ctx, who, "at most 65535 query heads");
     if (ldx < static_cast<uint64_t>(heads + 2 * c->kv_heads) * c->dim || (heads && ldq < static_cast<uint64_t>(heads) * c->dim)) return refuse(ctx, who, "rows overlap (ldx or ldq is too small)");

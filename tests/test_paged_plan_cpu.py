@@ -37,7 +37,8 @@ int main() {
         if (hf2q_cuda_pages_attend_scratch_bytes(&ctx, &c, &b, kv * group, window, sinks, &bytes) != HF2Q_OK) return printf("refused\n"), 1;
         if (bytes < 256 || bytes % 256) return printf("bytes %llu\n", (unsigned long long)bytes), 1;
         ctx.launches = 0;
-        const int32_t rc = hf2q_cuda_pages_attend(&ctx, nullptr, &c, &b, place, HF2Q_DT_F32, 1u << 30, kv * group, 1.0f, window, sinks, place, HF2Q_DT_F32, 1u << 30, place, bytes);
+        void* rows_at = max_new ? place : nullptr;                        // (arrays without rows have no address)
+        const int32_t rc = hf2q_cuda_pages_attend(&ctx, nullptr, &c, &b, rows_at, HF2Q_DT_F32, 1u << 30, kv * group, 1.0f, window, sinks, rows_at, HF2Q_DT_F32, 1u << 30, place, bytes);
         if (rc != HF2Q_OK || (ctx.launches == 0) != (max_new == 0)) return printf("call %d %d\n", rc, ctx.launches), 1;
         if (max_new == 0) continue;
         // the parts cover the most positions that a call can go through, in steps of every kernel, and the scratch holds them
