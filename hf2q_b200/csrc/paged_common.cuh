@@ -117,7 +117,10 @@ constexpr uint32_t step_ctas(uint32_t dim, bool codes, bool tall) { return dim =
 template <typename OUT> __device__ __forceinline__ OUT out_value(float v, bool& clipped);
 template <> __device__ __forceinline__ float out_value<float>(float v, bool&) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 out_value<__nv_bfloat16>(float v, bool&) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half out_value<__half>(float v, bool& clipped) { return panel_f16(v, clipped); }      // (the panel of a product that follows)
+template <> __device__ __forceinline__ __half out_value<__half>(float v, bool& clipped) {      // (the panel of a product that follows)
+    const __half h = panel_f16(v, clipped);
+    return v == v ? h : __float2half_rn(v);                               // (clipping alone would turn NaN into the lowest number)
+}
 
 // the checks that all entries share; 0 or the text of what is wrong
 inline const char* pages_error(const hf2q_pages* c) {
