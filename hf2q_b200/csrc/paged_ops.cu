@@ -8,6 +8,8 @@
 // 16 sequences 2.5 us, a launch.
 //
 // Copies.  Bound by bytes: 12 pages of 16 rows in 32 layers of codes, 26 MB, 4.4 us; 8192 rows in four layers of bf16, 269 MB, 45 us, 6.0 TB/s.
+#include <math_constants.h>
+
 #include "paged_common.cuh"
 #include "seq_common.cuh"
 
@@ -166,9 +168,11 @@ __global__ void __launch_bounds__(AP_WARPS * 32) append_kernel(Pool c, Batch b, 
         const size_t at = c.row(page, h - sh.heads - (is_k ? 0 : c.kv_heads), in_page);
         if constexpr (CODES) {
             float top = 0.f;
+            bool number = true;
 #pragma unroll
-            for (int j = 0; j < V; ++j) top = fmaxf(top, fabsf(e[j]));
+            for (int j = 0; j < V; ++j) { top = fmaxf(top, fabsf(e[j])); number &= e[j] == e[j]; }
             for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            if (!__all_sync(0xffffffffu, number)) top = CUDART_NAN_F;     // (a maximum leaves NaN out: the scale has to say it, codes cannot)
             const float inv = top > 0.f ? 127.0f / top : 0.f;
             uint32_t w = 0;
 #pragma unroll

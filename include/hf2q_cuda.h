@@ -957,7 +957,7 @@ typedef struct hf2q_rotary {
 } hf2q_rotary;
 /* Rows of x (f32 or bf16, ldx elements apart): queries [heads][dim], keys [kv_heads][dim], values [kv_heads][dim].  Queries are
  * turned and stored to q_out (f32 or bf16, rows ldq apart), keys are turned and stored with the values at their positions.
- * rotary NULL: nothing is turned. */
+ * Codes of a head with a NaN have a NaN scale.  rotary NULL: nothing is turned. */
 HF2Q_API int32_t hf2q_cuda_pages_append(hf2q_ctx* ctx, void* stream, const hf2q_pages* c, const hf2q_page_batch* b,
                                         const hf2q_rotary* rotary, const void* x, uint32_t x_dtype, uint32_t ldx,
                                         uint32_t heads, void* q_out, uint32_t q_dtype, uint32_t ldq);
