@@ -173,10 +173,11 @@ __global__ void __launch_bounds__(AP_WARPS * 32) append_kernel(Pool c, Batch b, 
             for (int j = 0; j < V; ++j) { top = fmaxf(top, fabsf(e[j])); number &= e[j] == e[j]; }
             for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             if (!__all_sync(0xffffffffu, number)) top = CUDART_NAN_F;     // (a maximum leaves NaN out: the scale has to say it, codes cannot)
-            const float inv = top > 0.f ? 127.0f / top : 0.f;
+            const float up = top < 0x1p-100f ? 0x1p100f : 1.0f;           // (127 / top would pass the range below 2^-121)
+            const float inv = top > 0.f ? 127.0f / (top * up) : 0.f;
             uint32_t w = 0;
 #pragma unroll
-            for (int j = 0; j < V; ++j) w |= (static_cast<uint32_t>(__float2int_rn(e[j] * inv)) & 0xffu) << (8 * j);
+            for (int j = 0; j < V; ++j) w |= (static_cast<uint32_t>(__float2int_rn(e[j] * up * inv)) & 0xffu) << (8 * j);
             int8_t* codes = static_cast<int8_t*>(is_k ? c.k : c.v) + at * DIM + V * lane;
             if constexpr (V == 4) *reinterpret_cast<uint32_t*>(codes) = w;
             else *reinterpret_cast<uint16_t*>(codes) = static_cast<uint16_t>(w);

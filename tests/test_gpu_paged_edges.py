@@ -1,4 +1,4 @@
-"""Calls over pages at the edges of what is allowed: no rows."""
+"""Calls over pages at the edges of what is allowed: no rows, the smallest numbers."""
 import pytest
 import torch
 
@@ -27,3 +27,21 @@ def test_a_batch_without_rows(gpu_ctx, max_length, held, dtype):
     cache.attend(0, batch, q, 4, out)
     gpu_ctx.check_status()
     assert torch.equal(cache.k.view(I8), before.view(I8))
+
+
+@pytest.mark.parametrize("size", [2.0 ** -119, 2.0 ** -122, 2.0 ** -126, 2.0 ** -135, 2.0 ** -149])
+def test_codes_of_the_smallest_numbers(gpu_ctx, size):
+    """127 / top is past the f32 range there.  A value is off by half a code, a code's own share of the scale's rounding (half of the smallest
+    number, 127 times over) and roundings in 32 bits."""
+    c = Pages([(30, 0)], 2, 1, 64, 16, I8, 2)
+    c.x.mul_(size)
+    cache, q = c.cache(gpu_ctx), torch.empty((30, 128), device="cuda")
+    cache.append(0, c.batch(gpu_ctx), None, c.x.cuda(), 2, q)
+    gpu_ctx.check_status()
+    p = torch.arange(30)
+    page, row = c.table[0, p // 16].long(), p % 16
+    for t, scale, heads in ((cache.k, cache.k_scale, slice(2, 4)), (cache.v, cache.v_scale, slice(4, 6))):
+        want = c.x.view(30, -1, 64)[:, heads].double()
+        got = t[0].cpu()[page, :, row].double() * scale[0].cpu()[page, :, row].double()[..., None]
+        unit = want.abs().amax(-1, keepdim=True) / 127
+        assert bool(((got - want).abs() <= 0.501 * unit + 127 * 2.0 ** -150 + 127 * 2.0 ** -23 * unit).all())
