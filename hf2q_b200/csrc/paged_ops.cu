@@ -97,10 +97,7 @@ __global__ void __launch_bounds__(AP_WARPS * 32) append_kernel(Pool c, Batch b, 
     pdl_wait();
     const uint32_t t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, all = sh.heads + 2 * c.kv_heads;
     const uint32_t s = sequence_of(b, t);
-    if (s == b.seqs) {                                                   // behind the last sequence (or in front of the first)
-        if (threadIdx.x == 0 && t < b.start[0]) atomicOr(status, STATUS_BAD_PAGE);
-        return;
-    }
+    if (s == b.seqs) return;                                             // in front of the first sequence or behind the last
     const Span span = span_of(b, c.shift, s);
     const bool held = t - span.row0 < span.rows && span.length + (t - span.row0) >= span.rows;       // it has a position (padding in front has none)
     const uint32_t pos = held ? span.length - span.rows + (t - span.row0) : 0;

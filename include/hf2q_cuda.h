@@ -937,7 +937,7 @@ typedef struct hf2q_pages {
 /* The rows of one call.  Sequence s owns rows start[s] .. start[s + 1] - 1 (possibly none) and holds length[s] positions, the new ones
  * included: its rows are the last of them, in order.  Position p is row p % page of page table[s][p / page].  The arrays are read on
  * the device, so that a captured call can be replayed on other values; the call itself is laid out for `rows` rows in all, at most
- * max_new rows and max_length positions of a sequence.  Rows behind start[seqs] are left as they were.  With more rows than positions
+ * max_new rows and max_length positions of a sequence.  Rows in front of start[0] or behind start[seqs] are left as they were.  With more rows than positions
  * the first rows are padding: they are not appended and see nothing (their attention is zero).  What does not fit (a
  * page number >= pages, a length above max_length or the table, more than max_new rows, starts that run
  * backwards or past `rows`) touches no memory outside the arrays and is reported by hf2q_cuda_check_status; the outputs of the

@@ -1,9 +1,9 @@
-"""Calls over pages at the edges of what is allowed: no rows, the smallest numbers."""
+"""Calls over pages at the edges of what is allowed: no rows, rows of nobody, the smallest numbers."""
 import pytest
 import torch
 
 from hf2q_b200 import paged
-from tests.paged_util import Pages
+from tests.paged_util import Pages, attention, close
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +45,27 @@ def test_codes_of_the_smallest_numbers(gpu_ctx, size):
         got = t[0].cpu()[page, :, row].double() * scale[0].cpu()[page, :, row].double()[..., None]
         unit = want.abs().amax(-1, keepdim=True) / 127
         assert bool(((got - want).abs() <= 0.501 * unit + 127 * 2.0 ** -150 + 127 * 2.0 ** -23 * unit).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, I8])
+@pytest.mark.parametrize("lengths", [[(1, 30), (1, 5000)], [(90, 40), (5, 3)], [(70, 5000)]])
+def test_rows_in_front_of_the_first_sequence_are_nobodys(gpu_ctx, lengths, dtype):
+    c = Pages(lengths, 2, 4, 64, 16, dtype, 3)
+    front, back, width = 3, 2, c.heads * 64
+    rows = front + c.rows + back
+    c.start += front
+    x = torch.randn((rows, c.x.shape[1]), generator=torch.Generator().manual_seed(1))
+    cache, batch, q, out = c.cache(gpu_ctx), c.batch(gpu_ctx, rows=rows), torch.full((rows, width), 7.0, device="cuda"), torch.full((rows, width), 7.0, device="cuda")
+    cache.attend(0, batch, torch.cat([torch.zeros((front, width)), c.q, torch.zeros((back, width))]).cuda(), c.heads, out)
+    gpu_ctx.check_status()
+    c.start -= front
+    want, tol = attention(c, c.q, F32, F32)
+    close(out[front:-back], want, tol)
+    assert bool((out[:front] == 7).all()) and bool((out[-back:] == 7).all())
+    cache.append(0, batch, None, x.cuda(), c.heads, q)
+    gpu_ctx.check_status()
+    assert torch.equal(q[front:-back].cpu(), x[front:-back, :width]) and bool((q[:front] == 7).all()) and bool((q[-back:] == 7).all())
+    p = int(c.length[0]) - 1                                          # the first sequence's last row went to its last position
+    got = cache.k[0, int(c.table[0, p // 16]), :, p % 16].cpu()
+    row = x[front + lengths[0][0] - 1].view(-1, 64)[c.heads:c.heads + 2]
+    assert torch.equal(got, row.to(BF)) if dtype == BF else torch.equal(got, (row * (127 / row.abs().amax(-1, keepdim=True))).round().to(I8))
