@@ -24,9 +24,11 @@ class PagedLlamaDecoder(LlamaDecoder):
         self.fused_attention = False
         i32 = dict(dtype=torch.int32, device=self.dev)
         self._q1 = torch.zeros((1, cfg.q_rows), dtype=torch.float32, device=self.dev)
-        self._row, self._len = torch.full((1, self.pages.table.shape[1]), -1, **i32), torch.zeros(1, **i32)    # of the bound sequence
+        # of the bound sequence: its pages; its length and the position that the newest token is turned by, pos + (1, shift)
+        self._row, self._at, self._plus = torch.full((1, self.pages.table.shape[1]), -1, **i32), torch.zeros(2, **i32), torch.tensor([1, 0], **i32)
+        self._len, self._turn = self._at[:1], self._at[1:]
         self._state = torch.zeros((n_slots, 2), **i32)                                                         # position and next token of the others
-        self._slot, self._portion = None, None
+        self._slot, self._portion, self._turns = None, None, None
         self._done = torch.cuda.Event()
         self._one = self._batch(1, cfg.max_seq)
         self._one.scratch(self.cache.structs[0], cfg.n_heads, 0, 0)                           # (before any capture)
@@ -98,6 +100,7 @@ class PagedLlamaDecoder(LlamaDecoder):
             raise RuntimeError("no sequence is bound")
         self.pages.reserve(self._slot, n)
         self._row.copy_(self.pages.table[self._slot:self._slot + 1])
+        self._plus[1:].fill_(self.pages.shift_of(self._slot))                            # (the pool may have compacted the sequence)
 
     def extend(self, slot: int, ids: torch.Tensor, want) -> torch.Tensor:
         self.bind(slot)
@@ -116,7 +119,7 @@ class PagedLlamaDecoder(LlamaDecoder):
             self._reserve(n)
             super().prefill(ids, start, want, want_out)
             self.pages.advance(self._slot, n)
-            self._portion = self._q = None
+            self._portion = self._q = self._turns = None
 
     def generate(self, n: int, use_graph: bool = True, collect: bool = True):
         """As ``LlamaDecoder.generate`` for the bound sequence."""
@@ -124,14 +127,14 @@ class PagedLlamaDecoder(LlamaDecoder):
             return torch.empty(0, dtype=torch.int32, device=self.dev) if collect else None
         with self._ordered():
             self._reserve(n)
-            self.pos.fill_(self.pages.length_of(self._slot))         # (the pool may have compacted the sequence)
+            self.pos.fill_(self.pages.length_of(self._slot))
             out = super().generate(n, use_graph, collect)
             self.pages.advance(self._slot, n)
         return out
 
     # ---- attention ------------------------------------------------------------------------------
     def decode_step(self) -> None:
-        torch.add(self.pos, 1, out=self._len)
+        torch.add(self.pos, self._plus, out=self._at)
         super().decode_step()
 
     @property
@@ -141,7 +144,7 @@ class PagedLlamaDecoder(LlamaDecoder):
 
     def _attend_step(self, i: int) -> None:
         c = self.cfg
-        self.cache.append(i, self._one, self.rope, self.qkv, c.n_heads, self._q1)
+        self.cache.append(i, self._one, self.rope, self.qkv, c.n_heads, self._q1, positions=self._turn)
         self.cache.attend(i, self._one, self._q1, c.n_heads, self.att)
 
     def _attend_portion(self, i: int, qkv, m: int, p0: int, att) -> None:
@@ -149,5 +152,7 @@ class PagedLlamaDecoder(LlamaDecoder):
         if i == 0:
             self._len.fill_(p0 + m)
             self._portion, self._q = self._batch(m, p0 + m), torch.empty((m, c.q_rows), dtype=torch.float32, device=self.dev)
-        self.cache.append(i, self._portion, self.rope, qkv, c.n_heads, self._q)
+            shift = self.pages.shift_of(self._slot)
+            self._turns = torch.arange(p0 + shift, p0 + shift + m, dtype=torch.int32, device=self.dev) if shift else None
+        self.cache.append(i, self._portion, self.rope, qkv, c.n_heads, self._q, positions=self._turns)
         self.cache.attend(i, self._portion, self._q, c.n_heads, att)

@@ -202,12 +202,27 @@ class PagedCache:
         self._move("hf2q_cuda_pages_copy_rows", src, dst)
 
 
+def _shifted(runs: list, keep: list) -> list:
+    """The runs (first place, position - place) of a sequence of which the places ``keep`` are left."""
+    out, k = [], 0
+    for i, p in enumerate(keep):
+        while k + 1 < len(runs) and runs[k + 1][0] <= p:
+            k += 1
+        shift = runs[k][1] + p - i
+        if not out or out[-1][1] != shift:
+            out.append((i, shift))
+    return out or [(0, 0)]
+
+
 class PagePool:
     """Which sequence owns which pages of a cache, kept on the host: pages are handed out lowest number first, branches of a sequence share
     them, and a shared page is copied before one of its owners writes into it.
 
     ``table`` [seqs, pages of max_length] and ``length`` [seqs] on the device follow the books, in the order of the current stream, for
-    ``PagedBatch`` to read."""
+    ``PagedBatch`` to read.
+
+    ``compact`` leaves keys turned by the positions that they had.  A sequence's next token is then turned by the position behind its last
+    key's, ``length_of + shift_of``, and not by its place (``append``'s ``positions``); ``shift`` [seqs] says so on the device."""
 
     def __init__(self, cache: PagedCache, seqs: int, max_length: int):
         if seqs < 1 or max_length < 1:
@@ -216,9 +231,11 @@ class PagePool:
         dev = cache.k.device
         self.table = torch.full((seqs, -(-max_length // cache.page)), -1, dtype=torch.int32, device=dev)
         self.length = torch.zeros(seqs, dtype=torch.int32, device=dev)
+        self.shift = torch.zeros(seqs, dtype=torch.int32, device=dev)
         self._free, self._refs = list(range(cache.pages)), [0] * cache.pages             # (a heap)
         self._pages: list = [None] * seqs                                                # page numbers of an open sequence
         self._lengths = [0] * seqs
+        self._shifts: list = [[(0, 0)] for _ in range(seqs)]                             # runs (first place, position - place), up to the next run's first place
 
     # ---- what the books say
     @property
@@ -231,6 +248,11 @@ class PagePool:
     def length_of(self, seq: int) -> int:
         self._own(seq)
         return self._lengths[seq]
+
+    def shift_of(self, seq: int) -> int:
+        """How far the position that the sequence's next token is turned by lies behind its place."""
+        self._own(seq)
+        return self._shifts[seq][-1][1]
 
     def _own(self, seq: int) -> list:
         if not 0 <= seq < self.seqs or self._pages[seq] is None:
@@ -267,19 +289,20 @@ class PagePool:
             self.table[seq, :len(pages)] = self._numbers(pages)
         self.table[seq, len(pages):].fill_(-1)
         self.length[seq:seq + 1].fill_(self._lengths[seq])
+        self.shift[seq:seq + 1].fill_(self._shifts[seq][-1][1])
 
     # ---- sequences
     def open(self) -> int:
         """A new sequence without positions."""
         seq = self._vacant()
-        self._pages[seq], self._lengths[seq] = [], 0
+        self._pages[seq], self._lengths[seq], self._shifts[seq] = [], 0, [(0, 0)]
         self._publish(seq)
         return seq
 
     def close(self, seq: int) -> None:
         """Gives the sequence's pages back, as far as no branch shares them."""
         self._drop(self._own(seq))
-        self._pages[seq], self._lengths[seq] = None, 0
+        self._pages[seq], self._lengths[seq], self._shifts[seq] = None, 0, [(0, 0)]
         self._publish(seq)
 
     def reserve(self, seq: int, n: int) -> None:
@@ -319,12 +342,13 @@ class PagePool:
         keep = pages[:-(-self._lengths[seq] // self.cache.page)]
         for p in keep:
             self._refs[p] += 1
-        self._pages[branch], self._lengths[branch] = list(keep), self._lengths[seq]
+        self._pages[branch], self._lengths[branch], self._shifts[branch] = list(keep), self._lengths[seq], list(self._shifts[seq])
         self._publish(branch)
         return branch
 
     def compact(self, seq: int, keep) -> None:
-        """Keeps the given positions (ascending) and packs them; the others are forgotten.  Keys stay turned as they are."""
+        """Keeps the given places (ascending) and packs them; the others are forgotten.  Keys stay turned as they are, and the sequence goes on
+        behind its last one (``shift_of``)."""
         pages, size = self._own(seq), self.cache.page
         keep = [int(p) for p in keep]
         if any(a >= b for a, b in zip(keep, keep[1:])) or (keep and (keep[0] < 0 or keep[-1] >= self._lengths[seq])):
@@ -337,7 +361,7 @@ class PagePool:
         if rest:
             self.cache.copy_rows(self._numbers([pages[p // size] * size + p % size for p in rest]), self._numbers([new[i // size] * size + i % size for i in range(len(rest))]))
         self._drop(pages[same:])
-        self._pages[seq], self._lengths[seq] = pages[:same] + new, len(keep)
+        self._pages[seq], self._lengths[seq], self._shifts[seq] = pages[:same] + new, len(keep), _shifted(self._shifts[seq], keep)
         self._publish(seq)
 
     def pack(self) -> int:

@@ -47,10 +47,10 @@ def quantize_kv(v: np.ndarray) -> np.ndarray:
     return (codes * scale).astype(np.float64)
 
 
-def forward(ids: np.ndarray, W: dict, cfg) -> np.ndarray:
+def forward(ids: np.ndarray, W: dict, cfg, hidden=None) -> np.ndarray:
     """Logits [T, vocab] of the prompt ``ids``; W maps tensor names to dequantised f32 matrices
     (token_embd, output, out_norm, blk.i.{attn_norm, attn_q, attn_k, attn_v, attn_output, ffn_norm,
-    ffn_gate, ffn_up, ffn_down})."""
+    ffn_gate, ffn_up, ffn_down}).  ``hidden`` [T, T]: places that a token does not see although they are in front of it."""
     T = len(ids)
     H, nh, nkv, d = cfg.hidden, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim
     g = nh // nkv
@@ -58,6 +58,8 @@ def forward(ids: np.ndarray, W: dict, cfg) -> np.ndarray:
     x = W["token_embd"][ids].astype(np.float64)
     f64 = lambda name: W[name].astype(np.float64)
     mask = np.triu(np.ones((T, T), dtype=bool), k=1)
+    if hidden is not None:
+        mask |= hidden
     for i in range(cfg.n_layers):
         p = f"blk.{i}."
         xn = rms_norm_rows(x, f64(p + "attn_norm"), cfg.rms_eps)

@@ -1,0 +1,60 @@
+"""The decoder after a compaction with holes: against the scalar forward in which the new tokens do not see what was forgotten and every token keeps
+its position."""
+import numpy as np
+import pytest
+import torch
+
+from hf2q_b200.decoder_paged import PagedLlamaDecoder
+from oracle import llama_forward
+from tests.test_gpu_decoder import CFG, LOGIT_GATE, build_model
+from tests.util import rel_l2
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def weights(gpu_ctx):
+    return build_model(gpu_ctx, CFG)
+
+
+def tokens(seed, n):
+    return torch.from_numpy(np.random.default_rng(seed).integers(0, CFG.vocab, size=n).astype(np.int32))
+
+
+@pytest.mark.parametrize("keep", [[*range(4), *range(110, 150)], [*range(0, 150, 3)], [*range(64), *range(100, 130)]], ids=["first-and-last", "every-third", "a-gap-and-no-end"])
+def test_tokens_behind_a_compaction(gpu_ctx, weights, keep):
+    """A portion through the panels, single tokens, and the captured step; a branch goes on as well; then the same once more."""
+    dec = PagedLlamaDecoder(gpu_ctx, CFG, weights[0], prefill_chunk=32, n_slots=2, pages=12)
+    ids, more = tokens(1, 150), tokens(2, 44)
+    s = dec.open_slot()
+    dec.extend(s, ids, [])
+    dec.pages.compact(s, keep)
+    n = keep[-1] + 1                                       # the position that the sequence goes on at
+    ids = torch.cat([ids[:n], more])
+    hidden = np.zeros((len(ids), len(ids)), dtype=bool)
+    hidden[n:, [p for p in range(n) if p not in keep]] = True
+    got = [dec.extend(s, more[:40], [0, 20, 39]), dec.extend(s, more[40:43], [2]), dec.extend(s, more[43:], [0])]
+    gpu_ctx.check_status()
+    want = llama_forward.forward(ids.numpy(), weights[1], CFG, hidden)
+    assert rel_l2(torch.cat(got).cpu().numpy(), want[[n, n + 20, n + 39, n + 42, n + 43]]) < LOGIT_GATE
+    branch = dec.fork(s)
+    for slot in (s, branch):
+        dec.bind(slot)
+        tok = int(dec.tok[0])
+        dec.generate(1)
+        wider = np.pad(hidden, ((0, 1), (0, 1)))
+        wider[-1] = np.append(hidden[-1], False)
+        want = llama_forward.forward(np.append(ids.numpy(), np.int32(tok)), weights[1], CFG, wider)[-1]
+        assert rel_l2(dec.logits.cpu().numpy()[0], want) < LOGIT_GATE
+    # once more: of what is left every second place, and the last one
+    left = [*keep, *range(n, n + 45)]
+    places = sorted({*range(0, len(left), 2), len(left) - 1})
+    dec.pages.compact(branch, places)
+    ids = torch.cat([ids, torch.tensor([tok], dtype=torch.int32), tokens(3, 2)])
+    gone = [p for p in range(n + 45) if p not in {left[i] for i in places}]
+    wider = np.pad(hidden, ((0, 3), (0, 3)))
+    wider[n + 44, :] = np.append(hidden[-1], [False] * 3)
+    wider[n + 45:, gone] = True
+    got = dec.extend(branch, ids[-2:], [0, 1])
+    gpu_ctx.check_status()
+    assert rel_l2(got.cpu().numpy(), llama_forward.forward(ids.numpy(), weights[1], CFG, wider)[-2:]) < LOGIT_GATE
