@@ -53,7 +53,7 @@ class PagedLlamaDecoder(LlamaDecoder):
     def _allocate_cache(self) -> None:
         c = self.cfg
         self.cache = paged.PagedCache.allocate(self.ctx, c.n_layers, self._n_pages, self.PAGE, c.n_kv_heads, c.head_dim, torch.int8)
-        self.pages = paged.PagePool(self.cache, self.n_slots, c.max_seq)
+        self.pages = paged.PagePool(self.cache, self.n_slots, c.max_seq, self._ordered)
 
     def _batch(self, m: int, max_length: int) -> paged.PagedBatch:
         """The bound sequence's last m tokens."""
@@ -82,6 +82,14 @@ class PagedLlamaDecoder(LlamaDecoder):
             branch = self.pages.fork(slot)
             self._state[branch] = torch.cat([self.pos, self.tok]) if slot == self._slot else self._state[slot]
         return branch
+
+    def compact(self, slot: int, keep) -> None:
+        """Keeps the given places of the sequence (ascending); the others are forgotten, and it goes on behind the last one."""
+        self.pages.compact(slot, keep)
+
+    def pack(self) -> int:
+        """Moves the sequences to the pool's lowest pages; returns how many are in use."""
+        return self.pages.pack()
 
     def bind(self, slot: int) -> None:
         self.pages.length_of(slot)                                                       # (raises for a slot that is not in use)

@@ -9,6 +9,8 @@ from __future__ import annotations
 import ctypes as C
 import heapq
 import math
+from contextlib import nullcontext
+from functools import wraps
 
 import torch
 
@@ -214,6 +216,14 @@ def _shifted(runs: list, keep: list) -> list:
     return out or [(0, 0)]
 
 
+def _in_order(method):
+    @wraps(method)
+    def call(self, *args, **kw):
+        with self._ordered():
+            return method(self, *args, **kw)
+    return call
+
+
 class PagePool:
     """Which sequence owns which pages of a cache, kept on the host: pages are handed out lowest number first, branches of a sequence share
     them, and a shared page is copied before one of its owners writes into it.
@@ -222,12 +232,14 @@ class PagePool:
     ``PagedBatch`` to read.
 
     ``compact`` leaves keys turned by the positions that they had.  A sequence's next token is then turned by the position behind its last
-    key's, ``length_of + shift_of``, and not by its place (``append``'s ``positions``); ``shift`` [seqs] says so on the device."""
+    key's, ``length_of + shift_of``, and not by its place (``append``'s ``positions``); ``shift`` [seqs] says so on the device.
 
-    def __init__(self, cache: PagedCache, seqs: int, max_length: int):
+    ``ordered``: a context manager that every call which reaches the device runs in, for owners whose calls come on several streams."""
+
+    def __init__(self, cache: PagedCache, seqs: int, max_length: int, ordered=nullcontext):
         if seqs < 1 or max_length < 1:
             _refuse("a pool serves 1 sequence or more, of 1 position or more")
-        self.cache, self.seqs, self.max_length = cache, seqs, max_length
+        self.cache, self.seqs, self.max_length, self._ordered = cache, seqs, max_length, ordered
         dev = cache.k.device
         self.table = torch.full((seqs, -(-max_length // cache.page)), -1, dtype=torch.int32, device=dev)
         self.length = torch.zeros(seqs, dtype=torch.int32, device=dev)
@@ -292,6 +304,7 @@ class PagePool:
         self.shift[seq:seq + 1].fill_(self._shifts[seq][-1][1])
 
     # ---- sequences
+    @_in_order
     def open(self) -> int:
         """A new sequence without positions."""
         seq = self._vacant()
@@ -299,12 +312,14 @@ class PagePool:
         self._publish(seq)
         return seq
 
+    @_in_order
     def close(self, seq: int) -> None:
         """Gives the sequence's pages back, as far as no branch shares them."""
         self._drop(self._own(seq))
         self._pages[seq], self._lengths[seq], self._shifts[seq] = None, 0, [(0, 0)]
         self._publish(seq)
 
+    @_in_order
     def reserve(self, seq: int, n: int) -> None:
         """Pages of its own for the sequence's next n positions (which ``advance`` then counts)."""
         pages, size, have = self._own(seq), self.cache.page, self._lengths[seq]
@@ -327,6 +342,7 @@ class PagePool:
         if new:
             self.table[seq, first:len(pages)] = self._numbers(pages[first:])
 
+    @_in_order
     def advance(self, seq: int, n: int) -> None:
         """The sequence has n more positions, in pages that ``reserve`` gave it."""
         pages, total = self._own(seq), self._lengths[seq] + n
@@ -335,6 +351,7 @@ class PagePool:
         self._lengths[seq] = total
         self.length[seq:seq + 1].fill_(total)
 
+    @_in_order
     def fork(self, seq: int) -> int:
         """A branch with the same positions: it shares the pages until one of the two writes."""
         pages = self._own(seq)
@@ -346,6 +363,7 @@ class PagePool:
         self._publish(branch)
         return branch
 
+    @_in_order
     def compact(self, seq: int, keep) -> None:
         """Keeps the given places (ascending) and packs them; the others are forgotten.  Keys stay turned as they are, and the sequence goes on
         behind its last one (``shift_of``)."""
@@ -364,6 +382,7 @@ class PagePool:
         self._pages[seq], self._lengths[seq], self._shifts[seq] = pages[:same] + new, len(keep), _shifted(self._shifts[seq], keep)
         self._publish(seq)
 
+    @_in_order
     def pack(self) -> int:
         """Moves pages to the lowest numbers; returns how many pages, from the front, are in use."""
         used = sorted(p for p, n in enumerate(self._refs) if n)

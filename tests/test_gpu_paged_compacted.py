@@ -58,3 +58,37 @@ def test_tokens_behind_a_compaction(gpu_ctx, weights, keep):
     got = dec.extend(branch, ids[-2:], [0, 1])
     gpu_ctx.check_status()
     assert rel_l2(got.cpu().numpy(), llama_forward.forward(ids.numpy(), weights[1], CFG, wider)[-2:]) < LOGIT_GATE
+
+
+@pytest.mark.parametrize("through", ["decoder", "pool"])
+def test_compaction_and_packing_wait_for_the_call_before(gpu_ctx, weights, through):
+    """On a stream of their own, directly behind a portion on another one."""
+    ids, keep = tokens(4, 400), [*range(4), *range(200, 400, 3)]
+
+    def run(streams):
+        dec = PagedLlamaDecoder(gpu_ctx, CFG, weights[0], prefill_chunk=400, n_slots=2, pages=20)
+        out = []
+        for _ in range(3):
+            a, b = dec.open_slot(), dec.open_slot()
+            calls = dec if through == "decoder" else dec.pages
+            with torch.cuda.stream(streams[0]):
+                dec.extend(a, tokens(5, 130), [])
+                dec.extend(b, ids, [])
+            with torch.cuda.stream(streams[1]):
+                calls.compact(b, keep)
+            with torch.cuda.stream(streams[2]):
+                dec.close_slot(a)
+                assert calls.pack() == 2
+            with torch.cuda.stream(streams[0]):
+                out.append(dec.extend(b, tokens(6, 9), [8]))
+            with torch.cuda.stream(streams[1]):
+                out.append(dec.generate(4))
+            torch.cuda.synchronize()
+            dec.close_slot(b)
+        gpu_ctx.check_status()
+        return out
+
+    here = torch.cuda.current_stream()
+    want = run([here, here, here])
+    got = run([torch.cuda.Stream() for _ in range(3)])
+    assert all(torch.equal(g, w) for g, w in zip(got, want))

@@ -49,3 +49,37 @@ def test_first_positions_and_the_last_ones():
     assert pool.length_of(s) + pool.shift_of(s) == 200
     pool.compact(s, range(4))                              # back to the first ones
     assert pool.length_of(s) + pool.shift_of(s) == 4
+
+
+def test_every_call_that_reaches_the_device_keeps_its_owners_order():
+    inside, calls = [], []
+
+    class Order:
+        def __enter__(self):
+            inside.append(1)
+
+        def __exit__(self, *error):
+            inside.pop()
+
+    class Watched(Contents):
+        def copy_rows(self, src, dst):
+            calls.append(bool(inside))
+            super().copy_rows(src, dst)
+
+    cache = Watched(12, 4)
+    pool = paged.PagePool(cache, 3, 40, Order)
+    plain = pool._publish
+    pool._publish = lambda seq: (calls.append(bool(inside)), plain(seq))
+    a = pool.open()
+    pool.reserve(a, 10)
+    pool.advance(a, 10)
+    b = pool.fork(a)
+    pool.reserve(b, 3)                                     # copies the page that both share
+    pool.advance(b, 3)
+    pool.compact(b, range(1, 13, 2))
+    pool.close(a)
+    pool.pack()
+    assert len(calls) >= 7 and all(calls) and not inside
+    with pytest.raises(RuntimeError):
+        pool.close(a)
+    assert not inside
