@@ -366,21 +366,55 @@ class PagePool:
     @_in_order
     def compact(self, seq: int, keep) -> None:
         """Keeps the given places (ascending) and packs them; the others are forgotten.  Keys stay turned as they are, and the sequence goes on
-        behind its last one (``shift_of``)."""
+        behind its last one (``shift_of``).  Forgetting an end moves nothing; else the places go to free pages, or where these do not suffice
+        to the front of the sequence's own, as far as no branch shares them."""
         pages, size = self._own(seq), self.cache.page
         keep = [int(p) for p in keep]
         if any(a >= b for a, b in zip(keep, keep[1:])) or (keep and (keep[0] < 0 or keep[-1] >= self._lengths[seq])):
             _refuse("positions to keep are ascending and among the sequence's own")
-        same = 0                                                                         # pages at the front that stay as they are
-        while (same + 1) * size <= len(keep) and keep[(same + 1) * size - 1] == (same + 1) * size - 1:
-            same += 1
-        rest = keep[same * size:]
-        new = self._take(-(-len(rest) // size))
-        if rest:
-            self.cache.copy_rows(self._numbers([pages[p // size] * size + p % size for p in rest]), self._numbers([new[i // size] * size + i % size for i in range(len(rest))]))
-        self._drop(pages[same:])
-        self._pages[seq], self._lengths[seq], self._shifts[seq] = pages[:same] + new, len(keep), _shifted(self._shifts[seq], keep)
+        n = len(keep)
+        if n == 0 or keep[-1] == n - 1:                                                  # only an end is forgotten: nothing moves
+            left = pages[:-(-n // size)]
+            self._drop(pages[len(left):])
+        else:
+            same = 0                                                                     # pages at the front that stay as they are
+            while (same + 1) * size <= n and keep[(same + 1) * size - 1] == (same + 1) * size - 1:
+                same += 1
+            need = -(-n // size) - same
+            own = set() if need <= len(self._free) else {j for j in range(same, same + need) if self._refs[pages[j]] == 1}
+            new = iter(self._take(need - len(own)))
+            left = pages[:same] + [pages[j] if j in own else next(new) for j in range(same, same + need)]
+            self._move_rows(pages, left, keep, same * size)
+            self._drop([p for j, p in enumerate(pages) if j >= same and j not in own])
+        self._pages[seq], self._lengths[seq], self._shifts[seq] = left, n, _shifted(self._shifts[seq], keep)
         self._publish(seq)
+
+    def _move_rows(self, pages: list, left: list, keep: list, first: int) -> None:
+        """Places ``keep[first:]`` of a sequence in ``pages`` become its places first, first + 1, .. in ``left``, where a page may stand that the
+        sequence had there before.  Places move to lower ones, so that in their order none is written before it was read.  A call has no
+        destination among its sources: it takes as many places as that allows, or goes by way of the free pages where they hold more."""
+        size = self.cache.page
+        row = lambda table, i: table[i // size] * size + i % size
+        moves = [(a, b) for a, b in ((row(pages, p), row(left, i)) for i, p in enumerate(keep[first:], first)) if a != b]
+        by, calls, at = [p * size + r for p in self._free[:-(-len(moves) // size)] for r in range(size)], [], 0
+        while at < len(moves):
+            read, written, end = set(), set(), at
+            while end < len(moves) and moves[end][0] not in written and moves[end][1] not in read:
+                read.add(moves[end][0])
+                written.add(moves[end][1])
+                end += 1
+            if end < len(moves) and end - at < len(by):
+                end = min(at + len(by), len(moves))
+                calls.append([(a, c) for (a, _), c in zip(moves[at:end], by)])
+                calls.append([(c, b) for (_, b), c in zip(moves[at:end], by)])
+            else:
+                calls.append(moves[at:end])
+            at = end
+        src, dst = (self._numbers([m[i] for call in calls for m in call]) for i in (0, 1))
+        at = 0
+        for call in calls:
+            self.cache.copy_rows(src[at:at + len(call)], dst[at:at + len(call)])
+            at += len(call)
 
     @_in_order
     def pack(self) -> int:

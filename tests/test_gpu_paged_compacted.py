@@ -92,3 +92,21 @@ def test_compaction_and_packing_wait_for_the_call_before(gpu_ctx, weights, throu
     want = run([here, here, here])
     got = run([torch.cuda.Stream() for _ in range(3)])
     assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+@pytest.mark.parametrize("keep", [range(1, 192), range(0, 192, 4), [*range(70), *range(75, 192)]], ids=["all-but-one", "every-fourth", "a-gap"])
+@pytest.mark.parametrize("more", [0, 1])
+def test_a_full_pool_gives_what_a_large_one_gives(gpu_ctx, weights, more, keep):
+    """Packed in the sequence's own pages (and through a free one), in all layers."""
+    got = []
+    for pages in (20, 3 + more):
+        dec = PagedLlamaDecoder(gpu_ctx, CFG, weights[0], prefill_chunk=192, n_slots=1, pages=pages)
+        s = dec.open_slot()
+        dec.extend(s, tokens(7, 192), [])
+        dec.compact(s, keep)
+        own = torch.tensor(dec.pages.pages_of(s), device="cuda")
+        at = torch.arange(len(keep), device="cuda")
+        rows = lambda t: t[:, own[at // 64], :, at % 64]
+        got.append([rows(t).clone() for t in (dec.cache.k, dec.cache.v, dec.cache.k_scale, dec.cache.v_scale)] + [dec.extend(s, tokens(8, 1), [0])])
+        gpu_ctx.check_status()
+    assert all(torch.equal(a, b) for a, b in zip(*got))

@@ -3,8 +3,8 @@ import random
 
 import pytest
 
-from hf2q_b200 import paged
-from tests.test_paged_cpu import Contents
+from hf2q_b200 import Hf2qError, paged
+from tests.test_paged_cpu import Contents, write
 
 
 @pytest.mark.parametrize("seed", range(5))
@@ -83,3 +83,90 @@ def test_every_call_that_reaches_the_device_keeps_its_owners_order():
     with pytest.raises(RuntimeError):
         pool.close(a)
     assert not inside
+
+
+def full(pages, size, more=0):
+    """A pool without a free page but ``more``: one sequence."""
+    cache = Contents(pages + more, size)
+    pool = paged.PagePool(cache, 3, (pages + more) * size)
+    return cache, pool, add(cache, pool, pool.open(), pages * size)
+
+
+def add(cache, pool, seq, n):
+    write(cache, pool, seq, list(range(n)))
+    return seq
+
+
+def holds(cache, pool, seq):
+    pages = pool.pages_of(seq)
+    assert len(set(pages)) == len(pages) and len(pages) == -(-pool.length_of(seq) // cache.page)
+    return [cache.rows[pages[i // cache.page] * cache.page + i % cache.page] for i in range(pool.length_of(seq))]
+
+
+@pytest.mark.parametrize("more", [0, 1])
+@pytest.mark.parametrize("keep", [range(0, 64, 4), range(60), range(1, 64), range(63), [*range(20), *range(21, 64)], [*range(32), *range(40, 64)], [63], [], range(64),
+                                  [*range(16), 63]])
+def test_a_full_pool_can_be_compacted(keep, more):
+    cache, pool, s = full(4, 16, more)
+    pool.compact(s, keep)
+    assert holds(cache, pool, s) == list(keep)
+    assert pool.n_free_pages == 4 + more - -(-len(keep) // 16)
+    pool.compact(s, range(pool.length_of(s)))
+    assert holds(cache, pool, s) == list(keep)
+
+
+def test_an_end_that_is_forgotten_moves_nothing():
+    """Rejected drafts: also where the pages are shared."""
+    cache, pool, s = full(4, 16)
+    pool.close(add(cache, pool, pool.fork(s), 0))
+    b = pool.fork(s)
+    cache.copy_rows = None
+    pool.compact(b, range(35))
+    assert holds(cache, pool, b) == list(range(35)) and pool.pages_of(b) == pool.pages_of(s)[:3] and pool.n_free_pages == 0
+    pool.compact(s, range(20))
+    assert holds(cache, pool, s) == list(range(20)) and pool.n_free_pages == 1
+
+
+def test_shared_pages_are_not_packed_in_place():
+    cache, pool, s = full(4, 16, 1)
+    b = pool.fork(s)
+    with pytest.raises(RuntimeError, match="no free page"):
+        pool.compact(b, range(1, 64))                      # four pages of its own
+    assert holds(cache, pool, b) == holds(cache, pool, s) == list(range(64))
+    pool.compact(b, range(1, 64, 5))
+    assert holds(cache, pool, b) == list(range(1, 64, 5)) and holds(cache, pool, s) == list(range(64)) and pool.n_free_pages == 0
+    pool.compact(s, range(1, 17))                          # s has its pages for itself now, and packs in them
+    assert holds(cache, pool, s) == list(range(1, 17))
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_compactions_of_pools_that_are_nearly_full(seed):
+    rnd = random.Random(seed)
+    size = rnd.choice([1, 4, 16])
+    cache = Contents(rnd.randrange(6, 20), size)
+    pool = paged.PagePool(cache, 3, cache.pages * size)
+    want = {pool.open(): [], pool.open(): []}
+    mark = 0
+    for _ in range(120):
+        s = rnd.choice(list(want))
+        n = rnd.randrange(0, size * cache.pages)
+        try:
+            write(cache, pool, s, list(range(mark, mark + n)))
+            want[s], mark = want[s] + list(range(mark, mark + n)), mark + n
+        except (RuntimeError, Hf2qError):
+            pass
+        if rnd.random() < 0.2 and len(want) < 3:
+            want[pool.fork(s)] = list(want[s])
+        part = rnd.choice([0.3, 0.9, 0.99])
+        keep = [i for i in range(len(want[s])) if rnd.random() < part]
+        try:
+            pool.compact(s, keep)
+            want[s] = [want[s][i] for i in keep]
+        except RuntimeError:
+            assert any(pool._refs[p] > 1 for p in pool.pages_of(s))
+        if rnd.random() < 0.1 and len(want) > 1:
+            pool.close(s)
+            del want[s]
+        for x, values in want.items():
+            assert holds(cache, pool, x)[:len(values)] == values and pool.length_of(x) == len(values)
+        assert pool.n_free_pages == cache.pages - len({p for x in want for p in pool.pages_of(x)})
