@@ -83,6 +83,10 @@ class PagedLlamaDecoder(LlamaDecoder):
             self._state[branch] = torch.cat([self.pos, self.tok]) if slot == self._slot else self._state[slot]
         return branch
 
+    def fits(self, lengths) -> bool:
+        """The free pages hold new sequences of these lengths, all at once."""
+        return sum(-(-n // self.PAGE) for n in lengths) <= self.pages.n_free_pages
+
     def compact(self, slot: int, keep) -> None:
         """Keeps the given places of the sequence (ascending); the others are forgotten, and it goes on behind the last one."""
         self.pages.compact(slot, keep)

@@ -46,20 +46,31 @@ class Engine:
         return (rows[0] if len(rows) == 1 else torch.cat(rows)) if rows else None
 
     def generate(self, prompts, n_new: int) -> list[list[int]]:
-        """Greedy continuations of the prompts (lists of token ids), n_new tokens each."""
+        """Greedy continuations of the prompts (lists of token ids), n_new tokens each.  As many prompts run at a time as there are slots and,
+        where the model's sequences share a pool, as fit it to their ends.  Slots are given back also if a call fails."""
         waiting = deque(enumerate(prompts))
         out: list = [None] * len(prompts)
+        fits = getattr(self.model, "fits", lambda lengths: True)
+        ends = [len(ids) + max(n_new - 1, 0) for ids in prompts]             # (the last token is not run)
+        for i, n in enumerate(ends):
+            if not fits([n]):
+                raise RuntimeError(f"prompt {i}: no room for {n} tokens, even alone")
         while waiting:
-            active = []
-            while waiting and len(active) < self.model.n_slots:
-                i, ids = waiting.popleft()
-                slot = self.model.open_slot()
-                self.model.extend(slot, torch.tensor(ids, dtype=torch.int32), [])
-                active.append((i, slot))
-            for i, slot in active:
-                self.model.bind(slot)
-                first = int(self.model.tok[0])
-                more = self.model.generate(n_new - 1).tolist() if n_new > 1 else []
-                out[i] = [first] + more
-                self.model.close_slot(slot)
+            group = [waiting.popleft()]
+            while waiting and len(group) < self.model.n_slots and fits([ends[i] for i, _ in [*group, waiting[0]]]):
+                group.append(waiting.popleft())
+            slots: list = []
+            try:
+                for _, ids in group:
+                    slots.append(self.model.open_slot())
+                    self.model.extend(slots[-1], torch.tensor(ids, dtype=torch.int32), [])
+                for i, _ in group:
+                    self.model.bind(slots[0])
+                    first = int(self.model.tok[0])
+                    more = self.model.generate(n_new - 1).tolist() if n_new > 1 else []
+                    out[i] = [first] + more
+                    self.model.close_slot(slots.pop(0))
+            finally:
+                for slot in slots:
+                    self.model.close_slot(slot)
         return out

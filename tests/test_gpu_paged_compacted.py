@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from hf2q_b200.decoder_paged import PagedLlamaDecoder
+from hf2q_b200.engine import Engine
 from oracle import llama_forward
 from tests.test_gpu_decoder import CFG, LOGIT_GATE, build_model
 from tests.util import rel_l2
@@ -110,3 +111,14 @@ def test_a_full_pool_gives_what_a_large_one_gives(gpu_ctx, weights, more, keep):
         got.append([rows(t).clone() for t in (dec.cache.k, dec.cache.v, dec.cache.k_scale, dec.cache.v_scale)] + [dec.extend(s, tokens(8, 1), [0])])
         gpu_ctx.check_status()
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_prompts_one_after_another_where_the_pool_holds_one(gpu_ctx, weights):
+    prompts = [tokens(9 + i, n).tolist() for i, n in enumerate((100, 70, 120))]
+    got = []
+    for slots, pages in ((3, 12), (2, 3)):
+        dec = PagedLlamaDecoder(gpu_ctx, CFG, weights[0], prefill_chunk=128, n_slots=slots, pages=pages)
+        got.append(Engine(dec).generate(prompts, 8))
+        assert dec.pages.n_free_pages == pages
+    gpu_ctx.check_status()
+    assert got[0] == got[1]
