@@ -18,6 +18,7 @@ graph and replayed once per generated token.
 from __future__ import annotations
 
 import ctypes as C
+import warnings
 from contextlib import contextmanager
 from dataclasses import dataclass
 
@@ -48,6 +49,15 @@ class LlamaConfig:
     @property
     def kv_rows(self) -> int:
         return self.n_kv_heads * self.head_dim
+
+
+def rotary_scaling(g) -> tuple:
+    """(kind, divisor of all turns, divisor of each pair's or None) of an open GGUF file with the ``llama`` key prefix."""
+    md = lambda k, default: g.metadata.get("llama.rope." + k, default)
+    old = float(md("scale_linear", 1.0))                     # (the key of earlier files)
+    kind = str(md("scaling.type", "none" if old == 1.0 else "linear"))
+    factors = g.load_tensor("rope_freqs.weight").view(np.float32).copy() if "rope_freqs.weight" in g.tensors else None
+    return kind, float(md("scaling.factor", old)) if kind == "linear" else 1.0, factors
 
 
 def use_more_bits(i_layer: int, n_layers: int) -> bool:
@@ -358,7 +368,13 @@ class LlamaDecoder(GreedyDecoder):
     @classmethod
     def from_gguf(cls, ctx: ops.GpuContext, path, max_seq: int = 32768, prefill_chunk: int = 2048) -> "LlamaDecoder":
         """Loads a GGUF file with the ``llama`` key prefix and tensor names (block bytes unchanged; an absent
-        output.weight means the tied embedding)."""
+        output.weight means the tied embedding).  This cache turns by rope.freq_base alone: for a file that scales its turns there is a
+        warning (``PagedLlamaDecoder`` scales them)."""
+        from .gguf import GgufFile
+        with GgufFile(path) as g:
+            kind, linear, factors = rotary_scaling(g)
+        if kind != "none" or linear != 1.0 or factors is not None:
+            warnings.warn(f"{path}: the file scales its rotary turns, and this cache does not; a cache in pages does (pages=)", stacklevel=2)
         return cls._load_gguf(ctx, path, max_seq, prefill_chunk, cls)
 
     @staticmethod

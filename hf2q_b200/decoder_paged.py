@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib, ops, paged
-from .decoder import LlamaConfig, LlamaDecoder, ModelWeights, SlotDecoder
+from .decoder import LlamaConfig, LlamaDecoder, ModelWeights, SlotDecoder, rotary_scaling
 
 
 class PagedLlamaDecoder(LlamaDecoder):
@@ -36,16 +36,17 @@ class PagedLlamaDecoder(LlamaDecoder):
     @classmethod
     def from_gguf(cls, ctx: ops.GpuContext, path, max_seq: int = 32768, prefill_chunk: int = 2048, *, n_slots: int = 4, pages: int | None = None) -> "PagedLlamaDecoder":
         """As ``LlamaDecoder.from_gguf``, with the turns scaled where the file says so (``rope_freqs.weight``: a divisor for each pair;
-        ``rope.scaling.factor`` of linear scaling).  ``pages`` None: room for every sequence at its longest."""
+        ``rope.scaling.factor`` of linear scaling); other scalings are refused.  ``pages`` None: room for every sequence at its longest."""
         from .gguf import GgufFile
         with GgufFile(path) as g:
-            factors = torch.from_numpy(g.load_tensor("rope_freqs.weight").view("f4").copy()) if "rope_freqs.weight" in g.tensors else None
-            linear = float(g.metadata.get("llama.rope.scaling.factor", 1.0)) if g.metadata.get("llama.rope.scaling.type") == "linear" else 1.0
+            kind, linear, factors = rotary_scaling(g)
+        if kind not in ("none", "linear"):
+            raise ops.Hf2qError(_lib.ERR_INVALID_ARGUMENT, f"rotary turns scaled by '{kind}' are not served (have: linear, a divisor for each pair)")
 
         def make(ctx, cfg, weights, prefill_chunk):
             freq = paged.rope_frequencies(cfg.head_dim, cfg.rope_theta, linear=linear)
             if factors is not None:
-                freq = (freq.double() / factors.double()).float()
+                freq = (freq.double() / torch.from_numpy(factors).double()).float()
             return cls(ctx, cfg, weights, prefill_chunk, n_slots=n_slots, pages=n_slots * -(-max_seq // cls.PAGE) if pages is None else pages, freq=freq)
 
         return cls._load_gguf(ctx, path, max_seq, prefill_chunk, make)

@@ -51,7 +51,8 @@ def architecture_of(path) -> str:
 
 def load_model(ctx: ops.GpuContext, path, dtype=torch.bfloat16, max_seq: int = 32768, n_slots: int = 1, prefill_chunk: int = 2048, pages: int | None = None):
     """The decoder that serves the model at ``path``: a folder with config.json and model.safetensors, or a .gguf file.  ``pages``: keep the
-    sequences of a quantized model, n_slots of them, in a pool of that many pages (None: one sequence in a cache of max_seq)."""
+    sequences of a quantized model, n_slots of them, in a pool of that many pages (None: one sequence in a cache of max_seq).  Only with pages
+    are rotary turns scaled as the file says; without them a file that scales its turns gives a warning."""
     arch = architecture_of(path)
     if arch not in ARCHITECTURES:
         raise ops.Hf2qError(_lib.ERR_INVALID_ARGUMENT, f"architecture '{arch}' is not registered (have: {', '.join(sorted(ARCHITECTURES))})")
