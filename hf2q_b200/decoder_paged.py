@@ -145,6 +145,15 @@ class PagedLlamaDecoder(LlamaDecoder):
             self.pages.advance(self._slot, n)
         return out
 
+    def _prefill_buffers(self, m, panels):
+        """As ``LlamaDecoder``'s; a stream that one call has used them on may still be at work when another call, on another stream, replaces them
+        by larger ones."""
+        have = super()._prefill_buffers(m, panels)
+        for t in have.values():
+            if isinstance(t, torch.Tensor):
+                t.record_stream(torch.cuda.current_stream(self.dev))
+        return have
+
     # ---- attention ------------------------------------------------------------------------------
     def decode_step(self) -> None:
         torch.add(self.pos, self._plus, out=self._at)

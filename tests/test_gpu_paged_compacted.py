@@ -122,3 +122,28 @@ def test_prompts_one_after_another_where_the_pool_holds_one(gpu_ctx, weights):
         assert dec.pages.n_free_pages == pages
     gpu_ctx.check_status()
     assert got[0] == got[1]
+
+
+def test_buffers_of_a_portion_stay_while_its_stream_works(gpu_ctx, weights):
+    """Made on one stream, used on a second one that is held up, replaced on a third one: what the first one allocates then is other memory."""
+    ids = tokens(20, 12 + 24 + 12 + 150)
+
+    def run(streams, hold):
+        dec = PagedLlamaDecoder(gpu_ctx, CFG, weights[0], prefill_chunk=256, n_slots=1, pages=8)
+        s, out, at = dec.open_slot(), [], 0
+        for i, n in enumerate((24, 12, 150)):
+            with torch.cuda.stream(streams[i]):
+                if hold and i == 1:
+                    torch.cuda._sleep(200_000_000)         # (a tenth of a second)
+                out.append(dec.extend(s, ids[at:at + n].cuda(), [n - 1]))
+            at += n
+        with torch.cuda.stream(streams[0]):
+            junk = [torch.full((rows, cols), float("nan"), device="cuda") for rows in (24,) for cols in (CFG.hidden, dec.qkv_cols, CFG.hidden // 2, CFG.q_rows // 2, CFG.ffn // 2) for _ in "ab"]
+        torch.cuda.synchronize()
+        gpu_ctx.check_status()
+        del junk
+        return out
+
+    here = torch.cuda.current_stream()
+    want = run([here] * 3, False)
+    assert all(torch.equal(a, b) for a, b in zip(run([torch.cuda.Stream() for _ in range(3)], True), want))
