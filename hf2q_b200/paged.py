@@ -346,7 +346,7 @@ class PagePool:
     def advance(self, seq: int, n: int) -> None:
         """The sequence has n more positions, in pages that ``reserve`` gave it."""
         pages, total = self._own(seq), self._lengths[seq] + n
-        if n < 0 or total > len(pages) * self.cache.page:
+        if n < 0 or total > min(len(pages) * self.cache.page, self.max_length):
             _refuse(f"{n} positions were not reserved")
         self._lengths[seq] = total
         self.length[seq:seq + 1].fill_(total)

@@ -170,3 +170,16 @@ def test_compactions_of_pools_that_are_nearly_full(seed):
         for x, values in want.items():
             assert holds(cache, pool, x)[:len(values)] == values and pool.length_of(x) == len(values)
         assert pool.n_free_pages == cache.pages - len({p for x in want for p in pool.pages_of(x)})
+
+
+def test_a_sequence_does_not_pass_the_pools_longest():
+    """6 positions in pages of 4: the last page has room for two that a batch of up to 6 would not take."""
+    pool = paged.PagePool(Contents(4, 4), 1, 6)
+    s = pool.open()
+    pool.reserve(s, 6)
+    with pytest.raises(Hf2qError):
+        pool.advance(s, 7)
+    pool.advance(s, 6)
+    with pytest.raises(Hf2qError):
+        pool.advance(s, 1)
+    assert pool.length_of(s) == 6
