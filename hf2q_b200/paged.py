@@ -49,8 +49,8 @@ def _rows(t: torch.Tensor, name: str, dtypes, rows: int, width: int, ctx) -> int
     right is seen with few questions.)"""
     if t.dtype in dtypes and t.get_device() == ctx.device and t.dim() == 2:
         (n, w), (ld, one) = t.shape, t.stride()
-        if n >= rows and w >= width and (one == 1 or w <= 1) and (ld >= width or rows <= 1):
-            return ld if rows > 1 else max(ld, width)
+        if n >= rows and w >= width and (one == 1 or w <= 1) and (rows <= 1 or width <= ld < 1 << 32):
+            return ld if rows > 1 else width
     _on_device(t, name, dtypes, ctx, contiguous=False)
     _refuse(f"{name} must hold {rows} rows of {width} elements side by side")
 

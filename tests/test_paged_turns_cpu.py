@@ -2,6 +2,7 @@
 import random
 
 import pytest
+import torch
 
 from hf2q_b200 import Hf2qError, paged
 from tests.test_paged_cpu import Contents, write
@@ -183,3 +184,15 @@ def test_a_sequence_does_not_pass_the_pools_longest():
     with pytest.raises(Hf2qError):
         pool.advance(s, 1)
     assert pool.length_of(s) == 6
+
+
+def test_rows_too_far_apart_for_the_entries_are_refused():
+    """A distance is passed in 32 bits."""
+    class OnCpu:
+        device = -1
+
+    rows = lambda n, apart: paged._rows(torch.empty((n, apart), device="meta")[:, :64], "x", (torch.float32,), n, 64, OnCpu())
+    assert rows(3, 70) == 70 and rows(3, (1 << 32) - 1) == (1 << 32) - 1
+    assert rows(1, 1 << 33) == 64                          # (one row has no distance)
+    with pytest.raises(Hf2qError):
+        rows(3, 1 << 32)
