@@ -81,6 +81,12 @@ def test_any_scale(gpu_ctx, lengths, scale, dtype):
     c.cache(gpu_ctx).attend(0, c.batch(gpu_ctx), c.q.to(BF).cuda(), c.heads, out, scale=scale)
     gpu_ctx.check_status()
     want, tol = attention(c, c.q, BF, F32, scale)
+    if dtype == I8:
+        # Where one score is far above the others their weights fall below the f16 normal range (2^-14), where a rounding is off by half of 2^-24.  Many
+        # rows: the weight of p is p * v_scale * 16 / U, U a power of two of at most twice the largest v_scale, so that p * v_scale is off by at
+        # most 2^-25 U / 16 = 2^-28 of the largest v_scale, for each position, times a code of up to 127, over a sum of at least 1.  (Few rows
+        # have 256 in the place of 16.)
+        tol = tol + int(c.length.max()) * 127 * c.v_scale.nan_to_num(0).max().double() * 2.0 ** -28
     close(out, want, tol)
 
 
