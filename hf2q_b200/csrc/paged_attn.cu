@@ -104,7 +104,7 @@ cudaError_t launch_join(const AttendCall& a) {
 // of up to 3001 30 / 22).
 constexpr uint64_t STEP_UNITS = 16, STEP_UNITS_CODES = 32, STEP_UNITS_MOST = 64, STEP_WORK = 1 << 17, STEP_WORK_CODES = 1 << 18;
 struct Plan {
-    bool step;
+    bool step, shrink;
     uint32_t chunk, chunks;
     uint64_t scratch;
 };
@@ -159,6 +159,7 @@ Plan plan_of(const hf2q_pages& c, const hf2q_page_batch& b, uint32_t heads, uint
     }
     p.chunks = static_cast<uint32_t>((seen + chunk - 1) / chunk);
     p.chunk = static_cast<uint32_t>(chunk);
+    p.shrink = p.chunks > 1 && b.seqs <= 32 && tiles * p.chunks <= static_cast<uint64_t>(sms) * (p.step ? step_ctas(c.dim, codes, units > 8) : 1);
     p.scratch = p.chunks > 1 && b.rows ? (static_cast<uint64_t>(b.rows) * heads * p.chunks * (c.dim + 2) * 4 + 255) / 256 * 256 : 256;
     return p;
 }
@@ -205,7 +206,7 @@ HF2Q_API int32_t hf2q_cuda_pages_attend(hf2q_ctx* ctx, void* stream, const hf2q_
     if (reinterpret_cast<uintptr_t>(scratch) % 256) return refuse(ctx, who, "scratch is 256-byte aligned");
     const OnDevice on(ctx_device(ctx));
     float* part = static_cast<float*>(scratch);
-    const AttendCall a{pool_of(c), batch_of(b), Look{window, sinks, scale * 1.4426950408889634f}, heads, q, q_dtype, ldq, out, out_dtype, ldo, p.chunk, p.chunks,
+    const AttendCall a{pool_of(c), batch_of(b), Look{window, sinks, scale * 1.4426950408889634f}, heads, q, q_dtype, ldq, out, out_dtype, ldo, p.chunk, p.chunks, p.shrink,
                        part, part + static_cast<size_t>(b->rows) * heads * p.chunks * c->dim, ctx_status_word(ctx), static_cast<cudaStream_t>(stream)};
     cudaError_t e = (p.step ? launch_attend_step : launch_attend_tiles)(a, c->dim, c->dtype == HF2Q_DT_I8);
     if (e == cudaSuccess && p.chunks > 1) e = c->dim == 128 ? launch_join<128>(a) : launch_join<64>(a);

@@ -91,6 +91,7 @@ struct AttendCall {
     void* out;
     uint32_t out_dtype, ldo;
     uint32_t chunk, chunks;                  // positions of a part, a multiple of 128
+    bool shrink;                             // parts follow the lengths
     float *part, *part_ml;                   // [rows][heads][chunks][dim], [rows][heads][chunks][2]
     uint32_t* status;
     cudaStream_t st;
@@ -103,9 +104,12 @@ __device__ __forceinline__ float part_factor(float m, float l, float m_all) { re
 
 // How many units of 2^log positions a part has.  A call is laid out for max_length; where up to 32 sequences are all much shorter now, their
 // parts are as much shorter, down to `least`, so that as many CTAs work.  (Whole warps come here.  Either number of units covers all: there
-// are `parts` times as many as the longest sequence has.)
-__device__ __forceinline__ uint32_t part_units(const Batch& b, uint32_t log, uint32_t planned, uint32_t parts, uint32_t least) {
-    if (parts <= 1 || b.seqs > 32) return planned;
+// are `parts` times as many as the longest sequence has.)  Only where all CTAs run at once (`shrink`): else more, shorter rounds take the place
+// of few.  (Codes, 8 KV heads, one token of each sequence, us with and without: 4 sequences of 2000 laid out for 32768 13 / 27, 1 of 2000 12 / 16, 8 of 1000 laid
+// out for 8000 12 / 19; more than one round: 32 of 2000 laid out for 32768 75 / 49, 16 of 1000 laid out for 8000 32 / 23, 8 of 10000 laid out for 32768 61 / 56.
+// 64 rows of each of 4 sequences of 4000 laid out for 16000 54 / 143.)
+__device__ __forceinline__ uint32_t part_units(const Batch& b, uint32_t log, uint32_t planned, uint32_t parts, uint32_t least, bool shrink) {
+    if (!shrink) return planned;
     const uint32_t lane = threadIdx.x & 31, longest = __reduce_max_sync(0xffffffffu, lane < b.seqs ? min(b.length[lane], b.max_length) : 0u);
     if (4ull * longest > 3ull * b.max_length) return planned;
     return min(planned, max(least, ((longest + (1u << log) - 1 >> log) + parts - 1) / parts));

@@ -72,7 +72,7 @@ constexpr uint32_t step_smem() { return WARPS * (TALL ? 16 : 8) * (DIM + 4) * 4;
 template <int DIM, bool CODES, bool TALL, typename Q, typename OUT>
 __global__ void __launch_bounds__(WARPS * 32, step_ctas(DIM, CODES, TALL))
 attend_step_kernel(Pool c, Batch b, Look look, uint32_t heads, uint32_t group, const Q* q, uint32_t ldq, bool wide_q, OUT* out, uint32_t ldo, uint32_t chunk_steps, uint32_t chunks,
-                   float* part, float* part_ml, uint32_t* status) {
+                   bool shrink, float* part, float* part_ml, uint32_t* status) {
     constexpr int R = TALL ? 16 : 8, KS = DIM / 16;                       // rows, contraction steps of a score
     constexpr int UE = CODES ? 16 : 8;                                    // elements of a 16-byte unit
     constexpr int KU = DIM / UE / 4;                                      // units of a key row in a lane
@@ -86,7 +86,7 @@ attend_step_kernel(Pool c, Batch b, Look look, uint32_t heads, uint32_t group, c
     const uint32_t s = blockIdx.z, kvh = blockIdx.x % c.kv_heads, tile = blockIdx.x / c.kv_heads, chunk = blockIdx.y;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, t = lane & 3;
     const Span span = span_of(b, c.shift, s);
-    const uint32_t part_steps = part_units(b, STEP_LOG, chunk_steps, chunks, 8);
+    const uint32_t part_steps = part_units(b, STEP_LOG, chunk_steps, chunks, 8, shrink);
     if (span.bad && threadIdx.x == 0 && blockIdx.x == 0 && chunk == 0) atomicOr(status, STATUS_BAD_PAGE);
     const uint32_t u0 = tile * R, units = span.rows * group;
     if (u0 >= units) return;
@@ -448,7 +448,7 @@ cudaError_t launch(const AttendCall& a) {
     const uint32_t group = a.heads / a.c.kv_heads, R = TALL ? 16 : 8, tiles = static_cast<uint32_t>((static_cast<uint64_t>(a.b.max_new) * group + R - 1) / R);
     const bool wide = reinterpret_cast<uintptr_t>(a.q) % (4 * sizeof(Q)) == 0 && a.ldq % 4 == 0;
     return launch_pdl(kern, dim3(tiles * a.c.kv_heads, a.chunks, a.b.seqs), dim3(WARPS * 32), smem, a.st, a.c, a.b, a.look, a.heads, group, static_cast<const Q*>(a.q), a.ldq, wide,
-                      static_cast<OUT*>(a.out), a.ldo, a.chunk >> STEP_LOG, a.chunks, a.part, a.part_ml, a.status);
+                      static_cast<OUT*>(a.out), a.ldo, a.chunk >> STEP_LOG, a.chunks, a.shrink, a.part, a.part_ml, a.status);
 }
 template <int DIM, bool CODES, bool TALL, typename Q>
 cudaError_t launch_out(const AttendCall& a) {

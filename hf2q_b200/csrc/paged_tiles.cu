@@ -132,7 +132,7 @@ template <typename Q> __device__ __forceinline__ void load8(const Q* p, bool wid
 struct Shape {
     uint32_t heads, group, inv_group, tokens;           // inv_group: r * inv_group >> 16 = r / group for r < 128; tokens of a tile
     uint32_t ldq, ldo, chunk_blocks, chunks;
-    bool wide_q;
+    bool wide_q, shrink;
 };
 
 // The sequence and the first token of CTA tile `index` (tiles of 2 * tokens tokens, the sequences one after the other); false: there is none.
@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(THREADS, 1) attend_tiles_kernel(Pool c, Batch 
     const bool any = end_tok > lost;
     const uint32_t first = any ? before + max(tok0, lost) : 0, last = any ? before + end_tok - 1 : 0;
     const Blocks blocks = blocks_of(look, first, last, BP_LOG);
-    const uint32_t part_blocks = part_units(b, BP_LOG, sh.chunk_blocks, sh.chunks, 4);
+    const uint32_t part_blocks = part_units(b, BP_LOG, sh.chunk_blocks, sh.chunks, 4, sh.shrink);
     const uint32_t lo = static_cast<uint32_t>(min(static_cast<uint64_t>(chunk) * part_blocks, static_cast<uint64_t>(blocks.count)));
     const uint32_t nb = any ? min(part_blocks, blocks.count - lo) : 0;
     if (nb == 0) {
@@ -715,7 +715,7 @@ cudaError_t launch(const AttendCall& a) {
     const uint64_t per = 2 * tokens, seqs = std::min(a.b.seqs, a.b.rows), tiles = std::min(a.b.rows / per + seqs, seqs * ((a.b.max_new + per - 1) / per));
     if (tiles * a.c.kv_heads > 0x7fffffffull) return cudaErrorInvalidValue;
     const bool wide = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.ldq % (16 / sizeof(Q)) == 0;
-    const Shape sh{a.heads, group, 65536 / group + 1, tokens, a.ldq, a.ldo, a.chunk >> BP_LOG, a.chunks, wide};
+    const Shape sh{a.heads, group, 65536 / group + 1, tokens, a.ldq, a.ldo, a.chunk >> BP_LOG, a.chunks, wide, a.shrink};
     return launch_pdl(kern, dim3(static_cast<uint32_t>(tiles) * a.c.kv_heads, a.chunks), dim3(THREADS), smem, a.st, a.c, a.b, a.look, sh, static_cast<const Q*>(a.q),
                       static_cast<OUT*>(a.out), a.part, a.part_ml, a.status);
 }

@@ -45,6 +45,8 @@ int main() {
         const paged::AttendCall& a = paged::last;
         const uint64_t seen = window ? std::min<uint64_t>(max_length, (uint64_t)window + max_new + sinks) : max_length;
         if (a.chunk == 0 || a.chunk % 128 || a.chunks == 0 || a.chunks > 256 || (uint64_t)a.chunk * a.chunks < seen) return printf("parts %u of %u\n", a.chunks, a.chunk), 1;
+        // parts follow the lengths only where all CTAs run at once (two on an SM at most)
+        if (a.shrink && (seqs > 32 || a.chunks == 1 || (uint64_t)a.chunks * kv * std::min(seqs, rows) > 2 * 148)) return printf("shrink\n"), 1;
         if (a.chunks > 1 && bytes < (uint64_t)rows * kv * group * a.chunks * (dim + 2) * 4) return printf("scratch\n"), 1;
     }
     printf("right\n");
