@@ -2,10 +2,11 @@
 //
 // Append.  A pair (a, b) at position p with frequency f becomes (a cos pf - b sin pf, a sin pf + b cos pf).  The angle of a far position
 // does not fit 32 bits (at position 10^6 half a unit in the last place of f32 is 0.03 rad), so that product, sine and cosine are
-// taken in 64 bits, once per pair and token, and rounded to f32 together; the turn itself is f32, each product and sum rounded by itself.
+// taken in 64 bits, once per pair and CTA (a CTA a token; few tokens share their heads among several), and rounded to f32 together; the turn
+// itself is f32, each product and sum rounded by itself.
 // Bytes: scale = amax / 127 over the head, code = the nearest whole number of value * (127 / amax).
-// Bound by bytes where there are many rows.  Measured (32 query heads of 8 KV heads, dim 128): three prompts of up to 2048 rows to codes 48 us, 4.6 TB/s; one token of
-// 16 sequences 2.5 us, a launch.
+// Bound by bytes where there are many rows.  Measured (32 query heads of 8 KV heads, dim 128): three prompts of up to 2048 rows to codes 49 us, 4.5 TB/s (47.5 without
+// a turn), to bf16 47.5 us; one token of 16 sequences 2.8 us, a launch.
 //
 // Copies.  Bound by bytes: 12 pages of 16 rows in 32 layers of codes, 26 MB, 4.4 us; 8192 rows in four layers of bf16, 269 MB, 45 us, 6.0 TB/s.
 #include <math_constants.h>

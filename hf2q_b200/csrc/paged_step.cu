@@ -13,16 +13,25 @@
 // (With the rows as M half of every product is empty for 8 rows and fewer, and each accumulator pair is moved into a group of four.)
 // Codes of keys enter as f16 subnormals, (code + 128) 2^-24, and 128 times the sum of q is taken off again; codes of values as f16 whole
 // numbers.  Their weights are p * v_scale * 256 / U with U a power of two above all value scales of the warp's steps so far, which
-// keeps them inside the f16 range whatever the scales are.  Loads of the next step are under way while this step's products run: the
+// keeps them inside the f16 range whatever the scales are; below its normal numbers p * v_scale is off by at most 2^-32 of the largest
+// value scale.  Loads of the next step are under way while this step's products run: the
 // next keys once the scores are done, the next values once the values are.
 //
-// Measured (32 query heads of 8 KV heads, dim 128): one token behind 131071 positions of codes 56 us, 4.9 TB/s; one token of each of 32 sequences of up to
-// 8192 positions of codes 80 us, 3.9 TB/s (the parts are as long as the longest sequence wants them, the others end early); with the rows as M these were 95
-// and 122 us.  One token behind 200 positions 5.7 us, of which the launch and the chain page number - key - score - value are nearly all.
+// Roundings.  The matrix instructions take 16-bit operands, so queries in f32 and the weights above the fraction are rounded to the type of their
+// product: f16 beside codes, bf16 beside bf16 pages (2^-11 and 2^-8 of each number at most).  The weights' sum below it, maxima and outputs
+// stay in f32.  Against 64 bits, root of the mean square over that of the result: bf16 pages and result 0.0021 to 0.0023, where the result's own rounding
+// makes 0.0017; codes and f16 result 0.0003, of which 0.0002; codes and bf16 result 0.0017, all of it.  Weights in two 16-bit halves would double the
+// products with the values to take off that last third.
+//
+// Measured (32 query heads of 8 KV heads, dim 128): one token behind 131071 positions of codes 57 us, 4.8 TB/s, of bf16 90 us, 5.9 TB/s; one token of each of 32
+// sequences of up to 8192 positions of codes 81 us, 3.9 TB/s, of bf16 126 us, 4.8 TB/s (the parts are as long as the longest sequence wants them, the
+// others end early); with the rows as M codes were 95 and 122 us.  One token behind 200 positions 6.2 us, of which the launch and the chain page
+// number - key - score - value are nearly all.
 #include <math_constants.h>
 
 #include <type_traits>
 
+#include "paged_bits.cuh"
 #include "paged_common.cuh"
 #include "tc_common.cuh"
 
@@ -44,12 +53,6 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-template <bool CODES> __device__ __forceinline__ uint32_t pack2(float a, float b) {
-    if constexpr (CODES) return tc::pack_h2(a, b);
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ bool holds_nonfinite(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
 
 // rows and columns of an 8 x 8 matrix of 16-bit numbers exchanged: lane 4 r + t holds columns 2 t, 2 t + 1 of row r
 __device__ __forceinline__ uint32_t transposed(uint32_t a) {
@@ -58,12 +61,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t a) {
     return d;
 }
 __device__ __forceinline__ float2 half_pair(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
-
-// a power of two above |v| (v finite), within what 2^12 / U can be
-__device__ __forceinline__ float unit_above(float v) {
-    const uint32_t e = (__float_as_uint(v) & 0x7f800000u) + 0x00800000u;
-    return fminf(fmaxf(__uint_as_float(e), 0x1p-100f), 0x1p100f);
-}
 
 template <int DIM, bool CODES, bool TALL>
 constexpr uint32_t step_smem() { return WARPS * (TALL ? 16 : 8) * (DIM + 4) * 4; }

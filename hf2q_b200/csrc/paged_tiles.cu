@@ -16,12 +16,15 @@
 //
 // Tensor memory: S 2 x 2 x 64 columns, O 2 x dim.  Codes: the scale of K multiplies the f32 score; the weight is p * v_scale * UNITS / U in f16, U
 // a power of two above all value scales of the blocks so far, which the loaders keep: it grows seldom, and the output is rescaled
-// with it.  What a row does not see gets weight 0 by selection, whatever its scales and scores are.  bf16 values
+// with it; below the f16 normal numbers p * v_scale is off by at most 2^-28 of the largest value scale.  What a row does not see gets weight 0 by selection, whatever its scales and scores are.  bf16 values
 // that are infinite or NaN in blocks that only some rows see would turn a weight of 0 into NaN: the loaders find them, hand zeros to the
 // product, and the rows that see them add them up one by one.
 //
-// Measured (32 query heads of 8 KV heads, dim 128): 4096 rows behind 12288 positions of codes 1.37 ms, 700 TFLOP/s or 0.42 of the matrix rate; six sequences of
-// up to 701 rows, window 2048, bf16 186 us, 530 TFLOP/s; 64 rows behind 32768 positions of codes 73 us.  A block takes a CTA 1.7 us with codes and 1.4
+// Queries and weights are rounded to the 16 bits that the products take, maxima, sums and outputs are f32, as in paged_step.cu; the errors
+// against 64 bits are the same there and here.
+//
+// Measured (32 query heads of 8 KV heads, dim 128): 4096 rows behind 12288 positions of codes 1.37 ms, 700 TFLOP/s or 0.42 of the matrix rate, of bf16 1.16 ms,
+// 830 TFLOP/s; six sequences of up to 701 rows, window 2048, bf16 188 us, 530 TFLOP/s; 64 rows behind 32768 positions of codes 75 us.  A block takes a CTA 1.7 us with codes and 1.4
 // with bf16, where its products alone are 0.6.  What the rest is, from copies with parts left out: shared memory (Q is read again for 64 columns, scales
 // are read by every warp; half of a round), and the chain from scores to weights to output of a tile, which two tiles hide only in part.  Blocks of
 // 128 positions read Q half as often but leave one S a tile: long prompts 3 % faster, windows and short parts 10 % slower.  Short calls
@@ -30,6 +33,7 @@
 
 #include <type_traits>
 
+#include "paged_bits.cuh"
 #include "paged_common.cuh"
 #include "tc_common.cuh"
 
@@ -48,10 +52,9 @@ template <int N> __device__ __forceinline__ void fewer_registers() { asm volatil
 constexpr uint32_t APART = 8;
 template <int DIM> constexpr uint32_t tiles_smem() { return 2 * ROWS * DIM * 2 + 2 * STAGES * BP * DIM * 2 + 1024; }
 
-__device__ __forceinline__ uint32_t claim_columns(uint32_t* slot) {       // by one warp; every other CTA of the SM gives its own back by itself
+__device__ __forceinline__ void claim_columns(uint32_t* slot) {           // by one warp; every other CTA of the SM gives its own back by itself
     tmem_alloc(slot, COLS);
     tmem_relinquish();
-    return 0;
 }
 __device__ __forceinline__ bool elected() {                               // one lane of a whole warp
     uint32_t yes;
@@ -81,15 +84,6 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t b
 }
 __device__ __forceinline__ void copies_close() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ bool holds_nonfinite(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
-__device__ __forceinline__ float unit_above(float v) {                    // a power of two above |v| (v finite), within what 2^12 / U can be
-    return fminf(fmaxf(__uint_as_float((__float_as_uint(v) & 0x7f800000u) + 0x00800000u), 0x1p-100f), 0x1p100f);
-}
-template <bool CODES> __device__ __forceinline__ uint32_t pack2(float a, float b) {
-    if constexpr (CODES) return pack_h2(a, b);
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
 template <bool CODES> __device__ __forceinline__ float2 unpack2(uint32_t w) {
     if constexpr (CODES) return __half22float2(*reinterpret_cast<const __half2*>(&w));
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));

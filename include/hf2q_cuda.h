@@ -965,7 +965,8 @@ HF2Q_API int32_t hf2q_cuda_pages_append(hf2q_ctx* ctx, void* stream, const hf2q_
  * head h reads KV head h / (heads / kv_heads).  Position j is visible to i when j <= i and, with window > 0, i - j < window or
  * j < sinks.  What a row does not see has no part in it, infinities and NaN included.  q f32 or
  * bf16, out f32, bf16 or f16 (beyond the f16 range clipped and noted in the status).  Codes are multiplied as exact f16 numbers
- * with q in f16 (clipped and noted), bf16 keys with q in bf16; probabilities are rounded to the same type, sums are f32.
+ * with q in f16 (clipped and noted), bf16 keys with q in bf16; probabilities are rounded to the same type, sums are f32.  Over codes a
+ * probability times its value scale is kept down to 2^-28 of the largest value scale that the rows see.
  * scratch: 256-byte aligned, of hf2q_cuda_pages_attend_scratch_bytes; its contents need not be kept. */
 HF2Q_API int32_t hf2q_cuda_pages_attend_scratch_bytes(hf2q_ctx* ctx, const hf2q_pages* c, const hf2q_page_batch* b, uint32_t heads,
                                                       uint32_t window, uint32_t sinks, uint64_t* out);
