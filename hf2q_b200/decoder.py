@@ -370,18 +370,18 @@ class LlamaDecoder(GreedyDecoder):
         """Loads a GGUF file with the ``llama`` key prefix and tensor names (block bytes unchanged; an absent
         output.weight means the tied embedding).  This cache turns by rope.freq_base alone: for a file that scales its turns there is a
         warning (``PagedLlamaDecoder`` scales them)."""
-        from .gguf import GgufFile
-        with GgufFile(path) as g:
-            kind, linear, factors = rotary_scaling(g)
-        if kind != "none" or linear != 1.0 or factors is not None:
-            warnings.warn(f"{path}: the file scales its rotary turns, and this cache does not; a cache in pages does (pages=)", stacklevel=2)
-        return cls._load_gguf(ctx, path, max_seq, prefill_chunk, cls)
+        def scaled(kind, linear, factors):
+            if kind not in ("none", "linear") or linear != 1.0 or factors is not None:
+                warnings.warn(f"{path}: the file scales its rotary turns, and this cache does not; a cache in pages does (pages=)", stacklevel=4)
+
+        return cls._load_gguf(ctx, path, max_seq, prefill_chunk, cls, scaled)
 
     @staticmethod
-    def _load_gguf(ctx: ops.GpuContext, path, max_seq: int, prefill_chunk: int, make):
-        """``make(ctx, cfg, weights, prefill_chunk)`` of what the file holds."""
+    def _load_gguf(ctx: ops.GpuContext, path, max_seq: int, prefill_chunk: int, make, scaled):
+        """``make(ctx, cfg, weights, prefill_chunk)`` of what the file holds; first ``scaled`` with what it says of its turns."""
         from .gguf import GgufFile
         with GgufFile(path) as g:
+            scaled(*rotary_scaling(g))
             md = lambda k, default=None: g.metadata.get("llama." + k, default)
             n_q, hidden = int(md("attention.head_count")), int(md("embedding_length"))
             emb = g.tensors["token_embd.weight"]

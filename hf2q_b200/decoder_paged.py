@@ -37,19 +37,21 @@ class PagedLlamaDecoder(LlamaDecoder):
     def from_gguf(cls, ctx: ops.GpuContext, path, max_seq: int = 32768, prefill_chunk: int = 2048, *, n_slots: int = 4, pages: int | None = None) -> "PagedLlamaDecoder":
         """As ``LlamaDecoder.from_gguf``, with the turns scaled where the file says so (``rope_freqs.weight``: a divisor for each pair;
         ``rope.scaling.factor`` of linear scaling); other scalings are refused.  ``pages`` None: room for every sequence at its longest."""
-        from .gguf import GgufFile
-        with GgufFile(path) as g:
-            kind, linear, factors = rotary_scaling(g)
-        if kind not in ("none", "linear"):
-            raise ops.Hf2qError(_lib.ERR_INVALID_ARGUMENT, f"rotary turns scaled by '{kind}' are not served (have: linear, a divisor for each pair)")
+        turns = {}
+
+        def scaled(kind, linear, factors):
+            if kind not in ("none", "linear"):
+                raise ops.Hf2qError(_lib.ERR_INVALID_ARGUMENT, f"rotary turns scaled by '{kind}' are not served (have: linear, a divisor for each pair)")
+            turns.update(linear=linear, factors=factors)
 
         def make(ctx, cfg, weights, prefill_chunk):
-            freq = paged.rope_frequencies(cfg.head_dim, cfg.rope_theta, linear=linear)
+            factors = turns["factors"]
+            freq = paged.rope_frequencies(cfg.head_dim, cfg.rope_theta, linear=turns["linear"])
             if factors is not None:
                 freq = (freq.double() / torch.from_numpy(factors).double()).float()
             return cls(ctx, cfg, weights, prefill_chunk, n_slots=n_slots, pages=n_slots * -(-max_seq // cls.PAGE) if pages is None else pages, freq=freq)
 
-        return cls._load_gguf(ctx, path, max_seq, prefill_chunk, make)
+        return cls._load_gguf(ctx, path, max_seq, prefill_chunk, make, scaled)
 
     def _allocate_cache(self) -> None:
         c = self.cfg

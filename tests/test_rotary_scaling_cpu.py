@@ -46,12 +46,14 @@ def test_other_scalings_are_refused_with_pages(tmp_path, keys):
         PagedLlamaDecoder.from_gguf(None, file(tmp_path, **keys))
 
 
-def test_a_cache_that_does_not_scale_says_so(tmp_path, monkeypatch):
-    monkeypatch.setattr(LlamaDecoder, "_load_gguf", staticmethod(lambda *a: "loaded"))
+def test_a_cache_that_does_not_scale_says_so(tmp_path):
+    """(The files have no weights: loading goes on behind the warning, and ends there.)"""
     for keys in [k for k, _ in SCALED] + OTHERS + [{"factors": [1.0, 2.0]}]:
-        with pytest.warns(UserWarning, match="scales its rotary turns"):
-            assert LlamaDecoder.from_gguf(None, file(tmp_path, **keys)) == "loaded"
+        with pytest.warns(UserWarning, match="scales its rotary turns") as seen, pytest.raises(TypeError):
+            LlamaDecoder.from_gguf(None, file(tmp_path, **keys))
+        assert seen[0].filename == __file__
     with warnings.catch_warnings():
         warnings.simplefilter("error")
-        for keys in PLAIN:
-            LlamaDecoder.from_gguf(None, file(tmp_path, **keys))
+        for keys in PLAIN + [{"scaling__type": "linear", "scaling__factor": 1.0}]:
+            with pytest.raises(TypeError):
+                LlamaDecoder.from_gguf(None, file(tmp_path, **keys))
